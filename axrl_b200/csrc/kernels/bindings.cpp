@@ -111,6 +111,12 @@ at::Tensor tc_linear_dgrad(at::Tensor dy, at::Tensor w);
 void adamw_p2p_step(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v, at::Tensor ptrs, int64_t s0, int64_t decay_end, double lr,
                     double b1, double b2, double eps, double wd, int64_t step, at::Tensor sqnorm, double clip, double extra_scale);
 void tc_linear_wgrad_acc(at::Tensor dy, at::Tensor x, at::Tensor acc, bool accumulate);
+std::vector<at::Tensor> qknorm_rope_cache_fp8(at::Tensor qkv, at::Tensor qw, at::Tensor kw, at::Tensor pos, at::Tensor inv_freq, int64_t nq,
+                                              int64_t nkv, double eps, at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor slots,
+                                              bool want_kv);
+void gather_kv_fp8(at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor slots, at::Tensor ko, at::Tensor vo);
+at::Tensor paged_decode_attn_fp8(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor block_table, at::Tensor seq_lens,
+                                 double scale);
 }  // namespace ax
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -214,4 +220,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tc_linear_dgrad", &ax::tc_linear_dgrad);
   m.def("adamw_p2p_step", &ax::adamw_p2p_step);
   m.def("tc_linear_wgrad_acc", &ax::tc_linear_wgrad_acc);
+  m.def("qknorm_rope_cache_fp8", &ax::qknorm_rope_cache_fp8);
+  m.def("gather_kv_fp8", &ax::gather_kv_fp8);
+  m.def("paged_decode_attn_fp8", &ax::paged_decode_attn_fp8);
 }
