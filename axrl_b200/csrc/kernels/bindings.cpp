@@ -117,6 +117,7 @@ std::vector<at::Tensor> qknorm_rope_cache_fp8(at::Tensor qkv, at::Tensor qw, at:
 void gather_kv_fp8(at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor slots, at::Tensor ko, at::Tensor vo);
 at::Tensor paged_decode_attn_fp8(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor block_table, at::Tensor seq_lens,
                                  double scale);
+int64_t kv_fp8_error();
 }  // namespace ax
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -223,4 +224,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qknorm_rope_cache_fp8", &ax::qknorm_rope_cache_fp8);
   m.def("gather_kv_fp8", &ax::gather_kv_fp8);
   m.def("paged_decode_attn_fp8", &ax::paged_decode_attn_fp8);
+  m.def("kv_fp8_error", &ax::kv_fp8_error);
 }

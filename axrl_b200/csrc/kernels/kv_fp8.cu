@@ -6,9 +6,12 @@
 // another token (the pages of a shared prefix stay as they are), and a power of two means that
 // code * scale is exact in bf16, so every reader sees the same values.  No counterpart in the reference
 // beyond its rollout engine's kv_cache_dtype option (axrl/configs.py RolloutWorkerConfig).
+#include <ATen/ops/zero.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <cuda.h>
 
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace ax {
 namespace kv8 {
@@ -188,67 +191,473 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 }
 
 // ----------------------------------------------------------------------------- decode
-// One CTA per (sequence, kv head); warp w takes tokens w, w + 8, ...; lane l holds dims 4l .. 4l + 3.
-// Online softmax per warp and q head, merged across the warps at the end.
-constexpr int DW = 8, MAXG = 16;
+// o = sum_t softmax_t(scale q.k_t) v_t with k_t = kc_t 2^{a_t}, v_t = vc_t 2^{e_t} (codes, exponents).
+//
+// Work: unit = 64 tokens of one (sequence, kv head).  The units of all (sequence, kv head) pairs in a row form
+// one list, cut into equal contiguous ranges, one per warp of the grid (one CTA per SM): every warp streams
+// the same number of bytes whatever the lengths are.  A pair that lies inside one range is finished by its warp; the
+// others leave fp32 partials (at most two per warp), which merge_k combines.  A warp works alone: its own ring
+// of 8 KB slots (K and V tiles in turn) filled by its own TMA loads (128-byte swizzle), no barrier with other warps.
+//
+// Per 16 tokens (m16n8k16, both operands f16, which holds every e4m3 code exactly):
+//   S^T (tokens x heads) = Kc Q^T     a lane reads 32 consecutive codes of its two token rows; the contraction index
+//                                      may be permuted freely as long as Q is read in the same order
+//   O^T (dims x heads)  += Vc^T P^T   a lane reads 16 consecutive codes of its four tokens; pairs of tokens are zipped
+//                                      byte by byte into the A fragment, so V needs no transposed load
+// P^T is the transpose (movmatrix) of the S^T fragment.  Up to eight q heads of a group fill the n = 8 columns (two
+// column tiles for groups of 9 to 16).
+//
+// Softmax in the log2 domain on w_t = scale log2(e) q.k_t + e_t, the exponent of V folded in: P_t = 2^{w_t - max w} <= 1
+// rounds to f16 (2^-11, finer than bf16) and multiplies the codes themselves; the normaliser is l = sum P_t 2^{-e_t} in
+// fp32, unrounded.  Whatever falls below f16 is 2^-24 of the largest weighted term.  q rows are scaled by a power of two
+// to [1, 2) before they are rounded to f16, which then only loses what is below 2^-25 of the row's largest.
+constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 3, TILE = UNIT * D;  // TILE: bytes of one slot
+constexpr int MAXB = 4096;
+constexpr int DEC_SMEM = 1024 + NW * SLOTS * TILE + NW * SLOTS * UNIT + NW * SLOTS * 8 + NW * SLOTS * 4 + (MAXB + 1) * 4;
 
-__global__ void __launch_bounds__(DW * 32) decode_k(const bf16* __restrict__ q, Cache c, const int* __restrict__ bt, const int* __restrict__ lens,
-                                                    bf16* __restrict__ out, int Hq, int max_pages, float scale_log2) {
-  __shared__ float sO[DW][D];
-  __shared__ float sM[DW][MAXG], sL[DW][MAXG];
-  const int b = blockIdx.x, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = Hq / c.Hkv;
-  const int len = (int)min((long)max(lens[b], 0), (long)max_pages * c.P);
-  float qf[MAXG][4], acc[MAXG][4], m[MAXG], l[MAXG];
-#pragma unroll
-  for (int g = 0; g < MAXG; ++g) {
-    m[g] = -INFINITY, l[g] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      qf[g][i] = g < G ? __bfloat162float(q[((long)b * Hq + hk * G + g) * D + 4 * lane + i]) : 0.f;
-      acc[g][i] = 0.f;
+__device__ int g_decode_err;  // first wait that gave up (0: none)
+
+struct DecParams {
+  const bf16* q;       // (B, Hq, 128)
+  const int* bt;       // (B, max_pages)
+  const int* lens;     // (B,)
+  const uint8_t *ks, *vs;
+  bf16* out;           // (B, Hq, 128)
+  float* part_o;       // (ranges, 2, G, 128)
+  float2* part_ml;     // (ranges, 2, G): max, sum
+  int* prefix;         // (B + 1): units of a kv head before sequence b, for merge_k
+  long pages;
+  int B, G, Hkv, P, max_pages, box;  // box: token rows of one TMA load, gcd(P, 64)
+  float scale_log2;
+};
+
+// Bounded wait for a tile; records that it gave up.
+__device__ __forceinline__ bool wait_tile(uint64_t* bar, uint32_t phase) {
+  for (long it = 0; !tc::mbar_try_wait(bar, phase); ++it)
+    if (it > tc::WAIT_LIMIT) {
+      atomicCAS(&g_decode_err, 0, 1);
+      return false;
     }
+  return true;
+}
+__device__ __forceinline__ int dec_len(const DecParams& p, int b) { return (int)min((long)max(p.lens[b], 0), (long)p.max_pages * p.P); }
+// First unit of range r of n over W units; n <= W, so no range is empty.
+__device__ __forceinline__ long range_lo(long r, long W, long n) { return r * W / n; }
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void bulk_bytes(void* dst, const void* src, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::s32(dst)), "l"(src), "r"(bytes), "r"(tc::s32(bar))
+               : "memory");
+}
+
+// The tile loads of one warp: K and V tiles of its range in turn, `SLOTS` ahead of their use.
+struct Loader {
+  int b, hk, u, U, len;  // unit that is loaded next
+  long left;             // units of the range still to load
+  int page, page_next;   // of this lane's chunk: page of the unit in flight, of the unit after it
+};
+
+template <int NT>
+__global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, DecParams p) {
+  extern __shared__ char smem_raw[];
+  char* sm = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  char* ring = sm + warp * SLOTS * TILE;
+  uint8_t* sc = reinterpret_cast<uint8_t*>(sm + NW * SLOTS * TILE) + warp * SLOTS * UNIT;  // scale bytes of a slot's tokens
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + NW * SLOTS * (TILE + UNIT)) + warp * SLOTS;
+  int* meta = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 8)) + warp * SLOTS;  // chunks of a slot that were loaded
+  int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12));
+  __shared__ int s_warp[NW];
+
+  if (lane == 0) {
+    for (int s = 0; s < SLOTS; ++s) tc::mbar_init(&full[s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  for (int t = warp; t < len; t += DW) {
-    const int page = bt[(long)b * max_pages + t / c.P];
-    if (page < 0 || page >= c.pages) continue;  // no such page: its tokens are not seen
-    const long row = ((long)page * c.Hkv + hk) * c.P + t % c.P;
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(c.k + row * D + 4 * lane), vw = *reinterpret_cast<const uint32_t*>(c.v + row * D + 4 * lane);
-    const float ks = scale_value(c.ks[row]) * scale_log2, vs = scale_value(c.vs[row]);
-    const float2 k0 = from_e4m3x2(kw), k1 = from_e4m3x2(kw >> 16), v0 = from_e4m3x2(vw), v1 = from_e4m3x2(vw >> 16);
+  pdl_trigger();
+  pdl_wait();
+  // exclusive prefix of the units of each sequence
+  {
+    const int per = (p.B + NW * 32 - 1) / (NW * 32), b0 = threadIdx.x * per;
+    int sum = 0;
+    for (int i = 0; i < per; ++i)
+      if (b0 + i < p.B) sum += (dec_len(p, b0 + i) + UNIT - 1) / UNIT;
+    int x = sum;
 #pragma unroll
-    for (int g = 0; g < MAXG; ++g) {
-      if (g >= G) break;
-      const float s = warp_sum(qf[g][0] * k0.x + qf[g][1] * k0.y + qf[g][2] * k1.x + qf[g][3] * k1.y) * ks;
-      const float mn = fmaxf(m[g], s), al = m[g] == -INFINITY ? 0.f : exp2f(m[g] - mn), p = exp2f(s - mn);
-      m[g] = mn;
-      l[g] = l[g] * al + p;
-      const float pv = p * vs;
-      acc[g][0] = acc[g][0] * al + pv * v0.x, acc[g][1] = acc[g][1] * al + pv * v0.y;
-      acc[g][2] = acc[g][2] * al + pv * v1.x, acc[g][3] = acc[g][3] * al + pv * v1.y;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-  }
-#pragma unroll
-  for (int g = 0; g < MAXG; ++g)
-    if (lane == 0) sM[warp][g] = m[g], sL[warp][g] = l[g];
-  __syncthreads();
-#pragma unroll
-  for (int g = 0; g < MAXG; ++g) {
-    if (g >= G) break;
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < DW; ++w) M = fmaxf(M, sM[w][g]);
-    for (int w = 0; w < DW; ++w) L += sM[w][g] == -INFINITY ? 0.f : sL[w][g] * exp2f(sM[w][g] - M);
-    const float f = m[g] == -INFINITY ? 0.f : exp2f(m[g] - M);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sO[warp][4 * lane + i] = acc[g][i] * f;
+    if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    if (threadIdx.x < D) {
-      float o = 0.f;
-      for (int w = 0; w < DW; ++w) o += sO[w][threadIdx.x];
-      out[((long)b * Hq + hk * G + g) * D + threadIdx.x] = __float2bfloat16(L == 0.f ? 0.f : o / L);
-    }
+    int before = x - sum;
+    for (int w = 0; w < warp; ++w) before += s_warp[w];
+    for (int i = 0; i < per; ++i)
+      if (b0 + i < p.B) {
+        prefix[b0 + i] = before;
+        before += (dec_len(p, b0 + i) + UNIT - 1) / UNIT;
+      }
+    if (threadIdx.x == NW * 32 - 1) prefix[p.B] = before;
     __syncthreads();
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i <= p.B; i += NW * 32) p.prefix[i] = prefix[i];
   }
+  const long W = (long)prefix[p.B] * p.Hkv;
+  const long nr = min((long)gridDim.x * NW, W);
+  const long r = (long)warp * gridDim.x + blockIdx.x;  // neighbouring ranges on different SMs: few units still use every SM
+  if (r >= nr) return;
+  const long x0 = range_lo(r, W, nr), n_units = range_lo(r + 1, W, nr) - x0;
+
+  int b, hk, u, U, len;  // unit that is worked on next
+  {
+    const int pos = (int)(x0 / p.Hkv);  // sequence b: prefix[b] <= pos < prefix[b + 1]
+    int lo = 0, hi = p.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= pos) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    U = prefix[b + 1] - prefix[b];
+    const int rem = (int)(x0 - (long)prefix[b] * p.Hkv);
+    hk = rem / U, u = rem % U;
+    len = dec_len(p, b);
+  }
+  const int chunks = UNIT / p.box;
+  Loader ld{b, hk, u, U, len, n_units, -1, -1};
+  auto page_of = [&](const Loader& x) {  // page of this lane's chunk of unit x, -1 if there is nothing to load
+    const int t = x.u * UNIT + lane * p.box;
+    if (lane >= chunks || t >= x.len) return -1;
+    const int pg = p.bt[(long)x.b * p.max_pages + t / p.P];
+    return pg < p.pages ? pg : -1;
+  };
+  auto advance = [&](Loader& x) {
+    if (++x.u < x.U) return;
+    x.u = 0;
+    if (++x.hk < p.Hkv) return;
+    x.hk = 0;
+    do ++x.b;
+    while (x.b < p.B - 1 && prefix[x.b + 1] == prefix[x.b]);
+    if (x.b < p.B) {
+      x.U = prefix[x.b + 1] - prefix[x.b];
+      x.len = dec_len(p, x.b);
+    }
+  };
+  auto issue = [&](int j, int page, const Loader& x) {  // tile j (even: K, odd: V) of unit x into slot j % SLOTS
+    const int s = j % SLOTS;
+    const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
+    if (lane == 0) {
+      meta[s] = (int)ok;
+      tc::mbar_expect_tx(&full[s], __popc(ok) * p.box * (D + 1));
+    }
+    __syncwarp();
+    if (page >= 0) {
+      const int t = x.u * UNIT + lane * p.box;
+      const int row = (int)(((long)page * p.Hkv + x.hk) * p.P) + t % p.P;
+      tc::tma_2d(ring + s * TILE + lane * p.box * D, (j & 1) ? &tv : &tk, 0, row, &full[s]);
+      bulk_bytes(sc + s * UNIT + lane * p.box, ((j & 1) ? p.vs : p.ks) + row, p.box, &full[s]);
+    }
+  };
+  // Loads run SLOTS tiles ahead: `nj` is the next tile to load, `ld` its unit.
+  int nj = 0;
+  Loader cur = ld;  // unit of the tile pair in flight (its V tile may still be to load)
+  ld.page_next = page_of(ld);
+  auto load_next = [&] {
+    if ((nj & 1) == 0) {
+      if (ld.left == 0) return;
+      cur = ld;
+      cur.page = ld.page_next;
+      --ld.left;
+      advance(ld);
+      ld.page_next = ld.left > 0 ? page_of(ld) : -1;
+    }
+    issue(nj, cur.page, cur);
+    ++nj;
+  };
+  __syncwarp();
+  for (int i = 0; i < SLOTS; ++i)
+    if (nj < 2 * n_units) load_next();
+
+  float acc[NT][8][4], m[NT][2], l[NT][2], qs[NT][2];
+  uint32_t qf[NT][16];
+  bool fresh = true;
+  const long first_u = u;  // the pair at the start of the range may have begun in an earlier one
+  bool begun_before = first_u > 0;
+  int j = 0;
+  for (long i = 0; i < n_units; ++i) {
+    if (fresh) {  // q fragments of this pair's heads
+      fresh = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int h = t * 8 + g;
+        uint4 w[4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          w[k] = h < p.G ? *reinterpret_cast<const uint4*>(p.q + (((long)b * p.Hkv + hk) * p.G + h) * D + 32 * c + 8 * k) : make_uint4(0, 0, 0, 0);
+          const uint32_t ws[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = max(top, max((ws[e] << 16) & 0x7fffffffu, ws[e] & 0x7fff0000u));
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        uint32_t ex = top >> 23;
+        if (ex == 0u || ex >= 254u) ex = 127u;
+        const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23) * p.scale_log2;
+        qs[t][0] = __shfl_sync(0xffffffffu, up, 8 * c);
+        qs[t][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t ws[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[t][4 * k + e] = pack_f16(__uint_as_float(ws[e] << 16) * down, __uint_as_float(ws[e] & 0xffff0000u) * down);
+        }
+        m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[t][d][0] = acc[t][d][1] = acc[t][d][2] = acc[t][d][3] = 0.f;
+      }
+    }
+    const int sk = j % SLOTS, sv = (j + 1) % SLOTS;
+    // --- K tile
+    bool ok = __all_sync(0xffffffffu, wait_tile(&full[sk], (j / SLOTS) & 1));
+    if (!ok) break;
+    const int loaded = meta[sk];
+    const int nval = min(UNIT, len - u * UNIT);
+    const bool partial = nval < UNIT || __popc(loaded) < chunks;
+    uint64_t seen = ~0ull;  // tokens of the unit that count
+    if (partial) {
+      seen = 0;
+      for (int k = 0; k < chunks; ++k)
+        if (loaded >> k & 1) seen |= (p.box == 64 ? ~0ull : ((1ull << p.box) - 1)) << (k * p.box);
+      if (nval < UNIT) seen &= (1ull << nval) - 1;
+    }
+    float s[NT][4][4];
+    float kf[4][2];
+    {
+      const char* kt = ring + sk * TILE;
+      const int o0 = ((2 * c) ^ g) << 4, o1 = ((2 * c + 1) ^ g) << 4;
+#pragma unroll
+      for (int i16 = 0; i16 < 4; ++i16) {
+        const char* r0 = kt + (i16 * 16 + g) * D;
+        const char* r1 = r0 + 8 * D;
+        const uint4 x0v = *reinterpret_cast<const uint4*>(r0 + o0), x1v = *reinterpret_cast<const uint4*>(r0 + o1);
+        const uint4 y0v = *reinterpret_cast<const uint4*>(r1 + o0), y1v = *reinterpret_cast<const uint4*>(r1 + o1);
+        const uint32_t xs[8] = {x0v.x, x0v.y, x0v.z, x0v.w, x1v.x, x1v.y, x1v.z, x1v.w};
+        const uint32_t ys[8] = {y0v.x, y0v.y, y0v.z, y0v.w, y1v.x, y1v.y, y1v.z, y1v.w};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][i16][0] = s[t][i16][1] = s[t][i16][2] = s[t][i16][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t a0 = to_f16x2(xs[k] & 0xffffu), a1 = to_f16x2(ys[k] & 0xffffu), a2 = to_f16x2(xs[k] >> 16), a3 = to_f16x2(ys[k] >> 16);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16(s[t][i16], a0, a1, a2, a3, qf[t][2 * k], qf[t][2 * k + 1]);
+        }
+        kf[i16][0] = scale_value(sc[sk * UNIT + i16 * 16 + g]);
+        kf[i16][1] = scale_value(sc[sk * UNIT + i16 * 16 + 8 + g]);
+      }
+    }
+    __syncwarp();
+    load_next();
+    // --- scores: w = scale log2(e) q.k + e
+    ok = __all_sync(0xffffffffu, wait_tile(&full[sv], ((j + 1) / SLOTS) & 1));
+    if (!ok) break;
+    float inv[4][2];
+#pragma unroll
+    for (int i16 = 0; i16 < 4; ++i16)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int tok = i16 * 16 + hh * 8 + g;
+        const uint32_t byte = sc[sv * UNIT + tok];
+        const float e = byte == 255u ? __uint_as_float(0x7fffffffu) : (float)((int)byte - 127);
+        inv[i16][hh] = __uint_as_float((uint32_t)max((int)((254 - (int)byte) << 23), 0x400000));
+        const bool in = seen >> tok & 1;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const float w = fmaf(s[t][i16][2 * hh + cc], kf[i16][hh] * qs[t][cc], e);
+            s[t][i16][2 * hh + cc] = in ? w : -INFINITY;
+          }
+      }
+    uint32_t pf[NT][4][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float alpha[2], ref[2];
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i16 = 0; i16 < 4; ++i16) mx = fmaxf(mx, fmaxf(s[t][i16][cc], s[t][i16][2 + cc]));
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float mn = fmaxf(m[t][cc], mx);
+        ref[cc] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
+        alpha[cc] = ex2(m[t][cc] - ref[cc]);
+        m[t][cc] = mn;
+        l[t][cc] *= alpha[cc];
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[t][d][0] *= alpha[0], acc[t][d][1] *= alpha[1], acc[t][d][2] *= alpha[0], acc[t][d][3] *= alpha[1];
+      }
+#pragma unroll
+      for (int i16 = 0; i16 < 4; ++i16)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const float p0 = ex2(s[t][i16][2 * hh] - ref[0]), p1 = ex2(s[t][i16][2 * hh + 1] - ref[1]);
+          l[t][0] = fmaf(p0, inv[i16][hh], l[t][0]);
+          l[t][1] = fmaf(p1, inv[i16][hh], l[t][1]);
+          pf[t][i16][hh] = transpose8x8(pack_f16(p0, p1));
+        }
+    }
+    // --- V tile
+    {
+      const char* vt = ring + sv * TILE;
+#pragma unroll
+      for (int i16 = 0; i16 < 4; ++i16) {
+        uint32_t w[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int tok = i16 * 16 + 2 * c + (k & 1) + (k >> 1) * 8;
+          uint4 x = *reinterpret_cast<const uint4*>(vt + tok * D + ((g ^ (tok & 7)) << 4));
+          if (partial && !(seen >> tok & 1)) x = make_uint4(0, 0, 0, 0);  // may hold a NaN code: 0 x NaN
+          w[k][0] = x.x, w[k][1] = x.y, w[k][2] = x.z, w[k][3] = x.w;
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const uint32_t sel = (d & 1) ? 0x7362 : 0x5140;
+          const uint32_t x = __byte_perm(w[0][d >> 1], w[1][d >> 1], sel), y = __byte_perm(w[2][d >> 1], w[3][d >> 1], sel);
+          const uint32_t a0 = to_f16x2(x & 0xffffu), a1 = to_f16x2(x >> 16), a2 = to_f16x2(y & 0xffffu), a3 = to_f16x2(y >> 16);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16(acc[t][d], a0, a1, a2, a3, pf[t][i16][0], pf[t][i16][1]);
+        }
+      }
+    }
+    __syncwarp();
+    load_next();
+    j += 2;
+    // --- end of the pair, or of the range
+    const bool ends = u == U - 1;
+    if (ends || i == n_units - 1) {
+      const bool whole = ends && !begun_before;
+      const long slot = (r * 2 + (begun_before ? 0 : 1)) * p.G;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          float sum = l[t][cc];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          const int h = t * 8 + 2 * c + cc;
+          if (h < p.G) {
+            if (whole) {
+              const float rl = sum == 0.f ? 0.f : 1.f / sum;
+              bf16* dst = p.out + (((long)b * p.Hkv + hk) * p.G + h) * D + 16 * g;
+              float f[8];
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) f[2 * d] = acc[t][4 * half + d][cc] * rl, f[2 * d + 1] = acc[t][4 * half + d][2 + cc] * rl;
+                store8(dst + 8 * half, f);
+              }
+            } else {
+              float* dst = p.part_o + (slot + h) * D + 16 * g;
+#pragma unroll
+              for (int d = 0; d < 4; ++d)
+                *reinterpret_cast<float4*>(dst + 4 * d) = make_float4(acc[t][2 * d][cc], acc[t][2 * d][2 + cc], acc[t][2 * d + 1][cc], acc[t][2 * d + 1][2 + cc]);
+              if (g == 0) p.part_ml[slot + h] = make_float2(m[t][cc], sum);
+            }
+          }
+        }
+      fresh = true;
+      begun_before = false;
+    }
+    if (++u == U) {
+      u = 0;
+      if (++hk == p.Hkv) {
+        hk = 0;
+        do ++b;
+        while (b < p.B - 1 && prefix[b + 1] == prefix[b]);
+        if (b < p.B) U = prefix[b + 1] - prefix[b], len = dec_len(p, b);
+      }
+    }
+  }
+  // after a wait that gave up: let the copies in flight land before the CTA's memory is released
+  for (; j < nj; ++j) wait_tile(&full[j % SLOTS], (j / SLOTS) & 1);
+}
+
+// The pairs that more than one range holds: out = sum_r 2^{m_r - M} o_r / sum_r 2^{m_r - M} l_r; zeros for empty sequences.
+// One warp per (sequence, q head).
+__global__ void __launch_bounds__(128) merge_k(DecParams p, long ranges) {
+  pdl_trigger();
+  pdl_wait();
+  const long w = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31, Hq = p.Hkv * p.G;
+  if (w >= (long)p.B * Hq) return;
+  const int b = (int)(w / Hq), h = (int)(w % Hq), hk = h / p.G;
+  const long U = p.prefix[b + 1] - p.prefix[b];
+  float4 o = make_float4(0, 0, 0, 0);
+  if (U > 0) {
+    const long W = (long)p.prefix[p.B] * p.Hkv, nr = min(ranges, W);
+    const long x0 = (long)p.prefix[b] * p.Hkv + hk * U;
+    const long r0 = ((x0 + 1) * nr - 1) / W, r1 = ((x0 + U) * nr - 1) / W;  // ranges of its first and last unit
+    if (r0 == r1) return;  // finished by its warp
+    float M = -INFINITY;
+    const long first = (r0 * 2 + 1) * p.G + h % p.G;  // then (r * 2) * G + head
+    for (long r = r0 + lane; r <= r1; r += 32) M = fmaxf(M, p.part_ml[r == r0 ? first : r * 2 * p.G + h % p.G].x);
+    M = warp_max(M);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+#pragma unroll 4
+    for (long r = r0; r <= r1; ++r) {
+      const long i = r == r0 ? first : r * 2 * p.G + h % p.G;
+      const float2 ml = p.part_ml[i];
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + i * D + 4 * lane);
+      const float f = ex2(ml.x - ref);
+      L = fmaf(f, ml.y, L);
+      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+    }
+    const float rl = L == 0.f ? 0.f : 1.f / L;
+    o.x *= rl, o.y *= rl, o.z *= rl, o.w *= rl;
+  }
+  bf16* dst = p.out + w * D + 4 * lane;
+  *reinterpret_cast<bf162*>(dst) = __floats2bfloat162_rn(o.x, o.y);
+  *reinterpret_cast<bf162*>(dst + 2) = __floats2bfloat162_rn(o.z, o.w);
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// A cache tensor as (pages Hkv P) rows of 128 codes; boxes of `box` rows, 128-byte swizzle.
+static CUtensorMap codes_map(const void* base, long rows, int box) {
+  static EncodeFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    AX_CHECK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && ptr, "cuTensorMapEncodeTiled");
+    return reinterpret_cast<EncodeFn>(ptr);
+  }();
+  CUtensorMap m;
+  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)D};
+  const cuuint32_t bx[2] = {(cuuint32_t)D, (cuuint32_t)box}, estr[2] = {1, 1};
+  const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  AX_CHECK(r == CUDA_SUCCESS, "tensor map encode failed (", (int)r, ")");
+  return m;
 }
 
 static Cache checked(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs) {
@@ -333,14 +742,40 @@ at::Tensor paged_decode_attn_fp8(at::Tensor q, at::Tensor k, at::Tensor v, at::T
   AX_CHECK(seq_lens.device() == dev && seq_lens.scalar_type() == at::kInt && seq_lens.numel() == B && seq_lens.is_contiguous(), "seq_lens: contiguous int32 (B,)");
   AX_CHECK(c.P % 16 == 0 && c.P > 0, "page size must be a multiple of 16");
   aligned16(q, "q");
+  AX_CHECK((reinterpret_cast<uintptr_t>(ks.data_ptr()) & 15) == 0 && (reinterpret_cast<uintptr_t>(vs.data_ptr()) & 15) == 0, "fp8 cache: scales start on a 16-byte boundary");
+  AX_CHECK(B <= MAXB, "decode batch must be <= ", MAXB);
+  const long rows = c.pages * c.Hkv * c.P;
+  AX_CHECK(rows < (1L << 31), "fp8 cache: pages * Hkv * page size must be below 2^31");
+  AX_CHECK(B * (block_table.size(1) * c.P / UNIT + 1) < (1L << 31), "block_table: too many tokens");
   const c10::cuda::CUDAGuard guard(dev);
   auto out = at::empty_like(q);
   if (B == 0) return out;
-  decode_k<<<dim3((unsigned)B, (unsigned)c.Hkv), DW * 32, 0, stream()>>>((const bf16*)q.data_ptr(), c, block_table.data_ptr<int>(), seq_lens.data_ptr<int>(),
-                                                                         (bf16*)out.data_ptr(), (int)Hq, (int)block_table.size(1),
-                                                                         (float)(scale * 1.4426950408889634));
+  if (rows == 0 || block_table.size(1) == 0) return out.zero_();
+  const int G = (int)(Hq / c.Hkv), grid = num_sms();
+  const long ranges = (long)grid * NW;
+  // freed after the launches, so the memory is handed on in stream order (and belongs to the graph when captured)
+  auto part_o = at::empty({ranges * 2 * G * D}, q.options().dtype(at::kFloat)), part_ml = at::empty({ranges * 2 * G * 2}, part_o.options());
+  auto prefix = at::empty({B + 1}, q.options().dtype(at::kInt));
+  int box = 16;
+  while (box < 64 && c.P % (2 * box) == 0) box *= 2;
+  const CUtensorMap tk = codes_map(c.k, rows, box), tv = codes_map(c.v, rows, box);
+  const DecParams p{(const bf16*)q.data_ptr(), block_table.data_ptr<int>(), seq_lens.data_ptr<int>(), c.ks, c.vs, (bf16*)out.data_ptr(),
+                    part_o.data_ptr<float>(), (float2*)part_ml.data_ptr<float>(), prefix.data_ptr<int>(), c.pages, (int)B, G, c.Hkv, c.P,
+                    (int)block_table.size(1), box, (float)(scale * 1.4426950408889634)};
+  auto kern = G <= 8 ? decode_k<1> : decode_k<2>;
+  smem_attr((const void*)kern, DEC_SMEM);
+  launch_pdl(kern, dim3(grid), dim3(NW * 32), DEC_SMEM, stream(), tk, tv, p);
+  AX_LAUNCH_OK();
+  launch_pdl(merge_k, dim3((unsigned)((B * Hq + 3) / 4)), dim3(128), 0, stream(), p, ranges);
   AX_LAUNCH_OK();
   return out;
+}
+
+// 0, or the code of the first bounded wait of the decode kernel that gave up on the current device.
+int64_t kv_fp8_error() {
+  int v = 0;
+  AX_CUDA_OK(cudaMemcpyFromSymbol(&v, kv8::g_decode_err, sizeof(int)));
+  return v;
 }
 
 }  // namespace ax

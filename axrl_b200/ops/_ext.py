@@ -67,7 +67,7 @@ def load(name: str = "_C") -> ModuleType:
 
 
 # Kernel launches per extension entry point (entry points not listed launch one kernel).
-_KERNELS_PER_CALL = {"attn_bwd": 3, "paged_decode_attn": 2, "rmsnorm_bwd": 2, "logprob_fwd": 1, "gemm": 1, "sample_tokens": 2}
+_KERNELS_PER_CALL = {"attn_bwd": 3, "paged_decode_attn": 2, "paged_decode_attn_fp8": 2, "rmsnorm_bwd": 2, "logprob_fwd": 1, "gemm": 1, "sample_tokens": 2}
 _COUNT = {"launches": 0, "enabled": False}
 
 
@@ -128,11 +128,11 @@ def available() -> bool:
 
 def check_kernel_waits() -> None:
     """Raise if a kernel with bounded internal waits (tcgen05 attention forward / backward, the
-    hand-written tcgen05 GEMM) gave up on a wait since the process started: its outputs are then
+    hand-written tcgen05 GEMM, decode attention over the 8-bit cache) gave up on a wait since the process started: its outputs are then
     incomplete.  Synchronises the stream."""
     e = ext()
     codes = {"tcgen05 attention": int(e.attn_tc_error()), "tcgen05 attention backward": int(e.attn_bwd_tc_error()),
-             "tcgen05 GEMM": int(e.tc_linear_error())}
+             "tcgen05 GEMM": int(e.tc_linear_error()), "fp8 decode attention": int(e.kv_fp8_error())}
     bad = {k: v for k, v in codes.items() if v}
     if bad:
         raise RuntimeError(f"kernel wait timed out: {bad}")

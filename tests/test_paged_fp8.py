@@ -253,6 +253,10 @@ def _check_decode(q, cache, bt, lens, scale=None):
     got = pf.paged_decode_attention_fp8(q, cache, bt, lens, scale)
     assert got.dtype == q.dtype and got.shape == q.shape
     want, tol = _exact_decode(q, cache, bt, lens, D ** -0.5 if scale is None else scale)
+    if q.is_cuda:
+        from axrl_b200.ops import _ext
+
+        assert _ext.ext().kv_fp8_error() == 0
     bad = (got.double() - want).abs() > tol
     assert not bad.any(), (bad.nonzero()[:5].tolist(), float((got.double() - want).abs().max()))
     return got
