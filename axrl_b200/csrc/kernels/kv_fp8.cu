@@ -199,18 +199,20 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // others leave fp32 partials (at most two per warp), which merge_k combines.  A warp works alone: its own ring
 // of 8 KB slots (K and V tiles in turn) filled by its own TMA loads (128-byte swizzle), no barrier with other warps.
 //
-// Per 16 tokens (m16n8k16, both operands f16, which holds every e4m3 code exactly):
-//   S^T (tokens x heads) = Kc Q^T     a lane reads 32 consecutive codes of its two token rows; the contraction index
-//                                      may be permuted freely as long as Q is read in the same order
-//   O^T (dims x heads)  += Vc^T P^T   a lane reads 16 consecutive codes of its four tokens; pairs of tokens are zipped
-//                                      byte by byte into the A fragment, so V needs no transposed load
-// P^T is the transpose (movmatrix) of the S^T fragment.  Up to eight q heads of a group fill the n = 8 columns (two
-// column tiles for groups of 9 to 16).
+// Both products run on e4m3 operands as they lie in the cache (m16n8k32, fp32 sums), so no code is ever converted:
+//   S^T (tokens x columns) = Kc Q^T,   O^T (dims x columns) += Vc^T P^T   (ldmatrix transposes the V bytes)
+// The other factor is split into two e4m3 terms that take a column each: x = hi + lo / 32 with hi = e4m3(x) and
+// lo = e4m3(32 (x - hi)), both scaled so that hi fills e4m3's range.  A bf16 q has 8 significant bits and splits exactly
+// (but for what is below 2^-22 of the row's largest); P keeps 8 bits, the precision of a bf16 P (at most 2^-8 of each
+// probability, 2^-23 of the largest for small ones).  Eight columns are the hi and lo of four heads; groups of 5 to 16
+// heads take two or four column tiles.  With f16 operands instead, the conversions of the codes were 60 % of 1590
+// instructions a unit and bound the kernel (74.4 us for 64 sequences of 146k tokens, against 46 us of bytes).
+//
+// P^T is the transpose (movmatrix) of the S^T fragment: one register holds hi and lo of two tokens.  Rows of S^T map to
+// tokens so that these two lie 4 apart mod 8, which keeps both ldmatrix forms free of bank conflicts on swizzled tiles.
 //
 // Softmax in the log2 domain on w_t = scale log2(e) q.k_t + e_t, the exponent of V folded in: P_t = 2^{w_t - max w} <= 1
-// rounds to f16 (2^-11, finer than bf16) and multiplies the codes themselves; the normaliser is l = sum P_t 2^{-e_t} in
-// fp32, unrounded.  Whatever falls below f16 is 2^-24 of the largest weighted term.  q rows are scaled by a power of two
-// to [1, 2) before they are rounded to f16, which then only loses what is below 2^-25 of the row's largest.
+// multiplies the codes themselves, and the normaliser is l = sum P_t 2^{-e_t} in fp32, unrounded.
 constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 3, TILE = UNIT * D;  // TILE: bytes of one slot
 constexpr int MAXB = 4096;
 constexpr int DEC_SMEM = 1024 + NW * SLOTS * TILE + NW * SLOTS * UNIT + NW * SLOTS * 8 + NW * SLOTS * 4 + (MAXB + 1) * 4;
@@ -244,18 +246,28 @@ __device__ __forceinline__ int dec_len(const DecParams& p, int b) { return (int)
 // First unit of range r of n over W units; n <= W, so no range is empty.
 __device__ __forceinline__ long range_lo(long r, long W, long n) { return r * W / n; }
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four 8 x 16-byte matrices: the A fragment of 16 rows x 32 bytes.
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// Two 16 x 16-byte matrices, transposed: the A fragment of 16 columns x 32 rows.
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// x, y (|.| <= 256) as e4m3 pairs: hi in the low half, 32 times the remainder in the high half.
+__device__ __forceinline__ uint32_t split2(float x, float y) {
+  const uint32_t hi = to_e4m3x2(x, y);
+  const float2 h = from_e4m3x2(hi);
+  return hi | to_e4m3x2(fmaf(h.x, -32.f, 32.f * x), fmaf(h.y, -32.f, 32.f * y)) << 16;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -267,11 +279,12 @@ __device__ __forceinline__ void bulk_bytes(void* dst, const void* src, int bytes
                : "memory");
 }
 
-// The tile loads of one warp: K and V tiles of its range in turn, `SLOTS` ahead of their use.
+// Position of a warp's loads in its range.
 struct Loader {
   int b, hk, u, U, len;  // unit that is loaded next
-  long left;             // units of the range still to load
-  int page, page_next;   // of this lane's chunk: page of the unit in flight, of the unit after it
+  int left;              // units of the range still to load
+  int pi, off;           // this lane's chunk of that unit: index into the block table, token within the page
+  int page;              // its page, fetched ahead; -1: nothing to load
 };
 
 template <int NT>
@@ -322,7 +335,8 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
   const long nr = min((long)gridDim.x * NW, W);
   const long r = (long)warp * gridDim.x + blockIdx.x;  // neighbouring ranges on different SMs: few units still use every SM
   if (r >= nr) return;
-  const long x0 = range_lo(r, W, nr), n_units = range_lo(r + 1, W, nr) - x0;
+  const long x0 = range_lo(r, W, nr);
+  const int n_units = (int)(range_lo(r + 1, W, nr) - x0);
 
   int b, hk, u, U, len;  // unit that is worked on next
   {
@@ -339,107 +353,131 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     hk = rem / U, u = rem % U;
     len = dec_len(p, b);
   }
+  // lane `ch` < chunks loads the box of tokens [ch box, (ch + 1) box) of a unit
   const int chunks = UNIT / p.box;
-  Loader ld{b, hk, u, U, len, n_units, -1, -1};
-  auto page_of = [&](const Loader& x) {  // page of this lane's chunk of unit x, -1 if there is nothing to load
-    const int t = x.u * UNIT + lane * p.box;
-    if (lane >= chunks || t >= x.len) return -1;
-    const int pg = p.bt[(long)x.b * p.max_pages + t / p.P];
-    return pg < p.pages ? pg : -1;
+  const bool loads = lane < chunks;
+  const int pi0 = lane * p.box / p.P, off0 = lane * p.box % p.P;
+  auto fetch_page = [&](Loader& x) {
+    x.page = -1;
+    if (loads && x.u * UNIT + lane * p.box < x.len) {
+      const int pg = p.bt[(long)x.b * p.max_pages + x.pi];
+      x.page = pg < p.pages ? pg : -1;
+    }
   };
-  auto advance = [&](Loader& x) {
-    if (++x.u < x.U) return;
-    x.u = 0;
+  auto next_unit = [&](Loader& x) {
+    if (++x.u < x.U) {
+      x.off += UNIT;
+      while (x.off >= p.P) x.off -= p.P, ++x.pi;
+      return;
+    }
+    x.u = 0, x.pi = pi0, x.off = off0;
     if (++x.hk < p.Hkv) return;
     x.hk = 0;
     do ++x.b;
     while (x.b < p.B - 1 && prefix[x.b + 1] == prefix[x.b]);
-    if (x.b < p.B) {
-      x.U = prefix[x.b + 1] - prefix[x.b];
-      x.len = dec_len(p, x.b);
-    }
+    if (x.b < p.B) x.U = prefix[x.b + 1] - prefix[x.b], x.len = dec_len(p, x.b);
   };
-  auto issue = [&](int j, int page, const Loader& x) {  // tile j (even: K, odd: V) of unit x into slot j % SLOTS
-    const int s = j % SLOTS;
-    const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
+  Loader ld{b, hk, u, U, len, n_units, (int)(((long)u * UNIT + lane * p.box) / p.P), (int)(((long)u * UNIT + lane * p.box) % p.P), -1};
+  fetch_page(ld);
+  int nj = 0, row = -1;  // next tile to load (even: K, odd: V of the same unit), its cache row
+  auto load_next = [&] {
+    if ((nj & 1) == 0) {
+      if (ld.left == 0) return;
+      row = ld.page >= 0 ? (int)(((long)ld.page * p.Hkv + ld.hk) * p.P) + ld.off : -1;
+      if (--ld.left > 0) {
+        next_unit(ld);
+        fetch_page(ld);
+      }
+    }
+    const int s = nj % SLOTS;
+    const uint32_t ok = __ballot_sync(0xffffffffu, row >= 0);
     if (lane == 0) {
       meta[s] = (int)ok;
       tc::mbar_expect_tx(&full[s], __popc(ok) * p.box * (D + 1));
     }
     __syncwarp();
-    if (page >= 0) {
-      const int t = x.u * UNIT + lane * p.box;
-      const int row = (int)(((long)page * p.Hkv + x.hk) * p.P) + t % p.P;
-      tc::tma_2d(ring + s * TILE + lane * p.box * D, (j & 1) ? &tv : &tk, 0, row, &full[s]);
-      bulk_bytes(sc + s * UNIT + lane * p.box, ((j & 1) ? p.vs : p.ks) + row, p.box, &full[s]);
+    if (row >= 0) {
+      tc::tma_2d(ring + s * TILE + lane * p.box * D, (nj & 1) ? &tv : &tk, 0, row, &full[s]);
+      bulk_bytes(sc + s * UNIT + lane * p.box, ((nj & 1) ? p.vs : p.ks) + row, p.box, &full[s]);
     }
-  };
-  // Loads run SLOTS tiles ahead: `nj` is the next tile to load, `ld` its unit.
-  int nj = 0;
-  Loader cur = ld;  // unit of the tile pair in flight (its V tile may still be to load)
-  ld.page_next = page_of(ld);
-  auto load_next = [&] {
-    if ((nj & 1) == 0) {
-      if (ld.left == 0) return;
-      cur = ld;
-      cur.page = ld.page_next;
-      --ld.left;
-      advance(ld);
-      ld.page_next = ld.left > 0 ? page_of(ld) : -1;
-    }
-    issue(nj, cur.page, cur);
     ++nj;
   };
   __syncwarp();
-  for (int i = 0; i < SLOTS; ++i)
-    if (nj < 2 * n_units) load_next();
+  for (int i = 0; i < SLOTS; ++i) load_next();
 
-  float acc[NT][8][4], m[NT][2], l[NT][2], qs[NT][2];
-  uint32_t qf[NT][16];
-  bool fresh = true;
-  const long first_u = u;  // the pair at the start of the range may have begun in an earlier one
-  bool begun_before = first_u > 0;
+  // row x of S^T is token x, row 8 + x token 8 + (x ^ 4) of 16
+  const int tok_a = g, tok_b = 8 + (g ^ 4);
+  uint32_t k_off[4], v_off;  // this lane's ldmatrix rows within a tile
+  {
+    const int x = lane & 7, tok = (lane >> 3 & 1) ? 8 + (x ^ 4) : x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k_off[i] = tok * D + (((2 * i + (lane >> 4)) ^ (tok & 7)) << 4);
+    const int y = lane >> 1 & 7, tv16 = (lane & 1) ? 8 + (y ^ 4) : y;  // rows of V in the order of P's bytes
+    v_off = ((lane >> 4) * 16 + tv16) * D + ((tv16 & 7) << 4);
+  }
+  const uint32_t ring_a = tc::s32(ring);
+  float acc[NT][8][4], m[NT], l[NT], qs[NT];
+  uint32_t qf[NT][8];
+  bool fresh = true, begun_before = u > 0;  // the pair at the start of the range may have begun in an earlier one
   int j = 0;
-  for (long i = 0; i < n_units; ++i) {
-    if (fresh) {  // q fragments of this pair's heads
+  for (int i = 0; i < n_units; ++i) {
+    if (fresh) {  // q columns of this pair: column g is hi (even) or lo (odd) of head 4 t + g / 2
       fresh = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int h = t * 8 + g;
-        uint4 w[4];
+        const int h = 4 * t + (g >> 1);
+        uint2 w[8];
         uint32_t top = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          w[k] = h < p.G ? *reinterpret_cast<const uint4*>(p.q + (((long)b * p.Hkv + hk) * p.G + h) * D + 32 * c + 8 * k) : make_uint4(0, 0, 0, 0);
-          const uint32_t ws[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = max(top, max((ws[e] << 16) & 0x7fffffffu, ws[e] & 0x7fff0000u));
+        for (int k = 0; k < 8; ++k) {
+          w[k] = h < p.G ? *reinterpret_cast<const uint2*>(p.q + (((long)b * p.Hkv + hk) * p.G + h) * D + 16 * k + 4 * c) : make_uint2(0, 0);
+          top = max(top, max(max((w[k].x << 16) & 0x7fffffffu, w[k].x & 0x7fff0000u), max((w[k].y << 16) & 0x7fffffffu, w[k].y & 0x7fff0000u)));
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        uint32_t ex = top >> 23;
-        if (ex == 0u || ex >= 254u) ex = 127u;
-        const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23) * p.scale_log2;
-        qs[t][0] = __shfl_sync(0xffffffffu, up, 8 * c);
-        qs[t][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
+        // largest value to [128, 256); rows that are not finite poison their scores through the factor
+        const uint32_t ex = top >> 23;
+        const float down = ex < 8u ? 1.f : __uint_as_float((261u - min(ex, 254u)) << 23);
+        const float up = ex == 255u ? __uint_as_float(0x7fffffffu) : p.scale_log2 * (ex < 8u ? 1.f : __uint_as_float((ex - 7u) << 23));
+        qs[t] = __shfl_sync(0xffffffffu, up, 8 * c);  // head 4 t + c
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t ws[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qf[t][4 * k + e] = pack_f16(__uint_as_float(ws[e] << 16) * down, __uint_as_float(ws[e] & 0xffff0000u) * down);
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t x = split2(__uint_as_float(w[k].x << 16) * down, __uint_as_float(w[k].x & 0xffff0000u) * down);
+          const uint32_t y = split2(__uint_as_float(w[k].y << 16) * down, __uint_as_float(w[k].y & 0xffff0000u) * down);
+          qf[t][k] = __byte_perm(x, y, (g & 1) ? 0x7632 : 0x5410);
         }
-        m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
+        m[t] = -INFINITY, l[t] = 0.f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) acc[t][d][0] = acc[t][d][1] = acc[t][d][2] = acc[t][d][3] = 0.f;
       }
     }
     const int sk = j % SLOTS, sv = (j + 1) % SLOTS;
-    // --- K tile
-    bool ok = __all_sync(0xffffffffu, wait_tile(&full[sk], (j / SLOTS) & 1));
-    if (!ok) break;
-    const int loaded = meta[sk];
-    const int nval = min(UNIT, len - u * UNIT);
+    // --- scores of 64 tokens
+    if (!__all_sync(0xffffffffu, wait_tile(&full[sk], (j / SLOTS) & 1))) break;
+    const int nval = min(UNIT, len - u * UNIT), loaded = meta[sk];
     const bool partial = nval < UNIT || __popc(loaded) < chunks;
+    float s[NT][4][2], kf[4][2];
+#pragma unroll
+    for (int i16 = 0; i16 < 4; ++i16) {
+      float sa[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sa[t][0] = sa[t][1] = sa[t][2] = sa[t][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t a[4];
+        ldsm4(a, ring_a + sk * TILE + i16 * 16 * D + k_off[k]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma_e4m3(sa[t], a, qf[t][2 * k], qf[t][2 * k + 1]);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s[t][i16][0] = fmaf(sa[t][1], 0.03125f, sa[t][0]), s[t][i16][1] = fmaf(sa[t][3], 0.03125f, sa[t][2]);
+      kf[i16][0] = scale_value(sc[sk * UNIT + i16 * 16 + tok_a]);
+      kf[i16][1] = scale_value(sc[sk * UNIT + i16 * 16 + tok_b]);
+    }
+    __syncwarp();
+    load_next();
+    // --- w = scale log2(e) q.k + e, and 256 P = 2^{w - max w + 8}
+    if (!__all_sync(0xffffffffu, wait_tile(&full[sv], ((j + 1) / SLOTS) & 1))) break;
     uint64_t seen = ~0ull;  // tokens of the unit that count
     if (partial) {
       seen = 0;
@@ -447,106 +485,74 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         if (loaded >> k & 1) seen |= (p.box == 64 ? ~0ull : ((1ull << p.box) - 1)) << (k * p.box);
       if (nval < UNIT) seen &= (1ull << nval) - 1;
     }
-    float s[NT][4][4];
-    float kf[4][2];
-    {
-      const char* kt = ring + sk * TILE;
-      const int o0 = ((2 * c) ^ g) << 4, o1 = ((2 * c + 1) ^ g) << 4;
-#pragma unroll
-      for (int i16 = 0; i16 < 4; ++i16) {
-        const char* r0 = kt + (i16 * 16 + g) * D;
-        const char* r1 = r0 + 8 * D;
-        const uint4 x0v = *reinterpret_cast<const uint4*>(r0 + o0), x1v = *reinterpret_cast<const uint4*>(r0 + o1);
-        const uint4 y0v = *reinterpret_cast<const uint4*>(r1 + o0), y1v = *reinterpret_cast<const uint4*>(r1 + o1);
-        const uint32_t xs[8] = {x0v.x, x0v.y, x0v.z, x0v.w, x1v.x, x1v.y, x1v.z, x1v.w};
-        const uint32_t ys[8] = {y0v.x, y0v.y, y0v.z, y0v.w, y1v.x, y1v.y, y1v.z, y1v.w};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][i16][0] = s[t][i16][1] = s[t][i16][2] = s[t][i16][3] = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t a0 = to_f16x2(xs[k] & 0xffffu), a1 = to_f16x2(ys[k] & 0xffffu), a2 = to_f16x2(xs[k] >> 16), a3 = to_f16x2(ys[k] >> 16);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) mma_f16(s[t][i16], a0, a1, a2, a3, qf[t][2 * k], qf[t][2 * k + 1]);
-        }
-        kf[i16][0] = scale_value(sc[sk * UNIT + i16 * 16 + g]);
-        kf[i16][1] = scale_value(sc[sk * UNIT + i16 * 16 + 8 + g]);
-      }
-    }
-    __syncwarp();
-    load_next();
-    // --- scores: w = scale log2(e) q.k + e
-    ok = __all_sync(0xffffffffu, wait_tile(&full[sv], ((j + 1) / SLOTS) & 1));
-    if (!ok) break;
     float inv[4][2];
 #pragma unroll
     for (int i16 = 0; i16 < 4; ++i16)
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        const int tok = i16 * 16 + hh * 8 + g;
-        const uint32_t byte = sc[sv * UNIT + tok];
-        const float e = byte == 255u ? __uint_as_float(0x7fffffffu) : (float)((int)byte - 127);
+        const uint32_t byte = sc[sv * UNIT + i16 * 16 + (hh ? tok_b : tok_a)];
+        const float e = byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(0x4b000000u + byte) - 8388735.f;  // byte - 127
         inv[i16][hh] = __uint_as_float((uint32_t)max((int)((254 - (int)byte) << 23), 0x400000));
-        const bool in = seen >> tok & 1;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            const float w = fmaf(s[t][i16][2 * hh + cc], kf[i16][hh] * qs[t][cc], e);
-            s[t][i16][2 * hh + cc] = in ? w : -INFINITY;
-          }
+        for (int t = 0; t < NT; ++t) s[t][i16][hh] = fmaf(s[t][i16][hh], kf[i16][hh] * qs[t], e);
       }
-    uint32_t pf[NT][4][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float alpha[2], ref[2];
-#pragma unroll
-      for (int cc = 0; cc < 2; ++cc) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i16 = 0; i16 < 4; ++i16) mx = fmaxf(mx, fmaxf(s[t][i16][cc], s[t][i16][2 + cc]));
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float mn = fmaxf(m[t][cc], mx);
-        ref[cc] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
-        alpha[cc] = ex2(m[t][cc] - ref[cc]);
-        m[t][cc] = mn;
-        l[t][cc] *= alpha[cc];
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-        for (int d = 0; d < 8; ++d) acc[t][d][0] *= alpha[0], acc[t][d][1] *= alpha[1], acc[t][d][2] *= alpha[0], acc[t][d][3] *= alpha[1];
-      }
+    if (partial) {
 #pragma unroll
       for (int i16 = 0; i16 < 4; ++i16)
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const float p0 = ex2(s[t][i16][2 * hh] - ref[0]), p1 = ex2(s[t][i16][2 * hh + 1] - ref[1]);
-          l[t][0] = fmaf(p0, inv[i16][hh], l[t][0]);
-          l[t][1] = fmaf(p1, inv[i16][hh], l[t][1]);
-          pf[t][i16][hh] = transpose8x8(pack_f16(p0, p1));
-        }
+        for (int hh = 0; hh < 2; ++hh)
+          if (!(seen >> (i16 * 16 + (hh ? tok_b : tok_a)) & 1)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[t][i16][hh] = -INFINITY;
+          }
     }
-    // --- V tile
-    {
-      const char* vt = ring + sv * TILE;
+    uint32_t pf[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float mx = fmaxf(s[t][0][0], s[t][0][1]);
+#pragma unroll
+      for (int i16 = 1; i16 < 4; ++i16) mx = fmaxf(mx, fmaxf(s[t][i16][0], s[t][i16][1]));
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mx = fmaxf(m[t], mx);
+      const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen yet
+      const float alpha = ex2(m[t] - ref);
+      m[t] = mx;
+      l[t] *= alpha;
+      if (__any_sync(0xffffffffu, alpha != 1.f)) {
+        // accumulator columns 2c, 2c + 1 are hi and lo of this lane's head
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[t][d][0] *= alpha, acc[t][d][1] *= alpha, acc[t][d][2] *= alpha, acc[t][d][3] *= alpha;
+      }
+      const float shift = 8.f - ref;
 #pragma unroll
       for (int i16 = 0; i16 < 4; ++i16) {
-        uint32_t w[4][4];
+        const float pa = ex2(s[t][i16][0] + shift), pb = ex2(s[t][i16][1] + shift);
+        l[t] = fmaf(pa, inv[i16][0], l[t]);
+        l[t] = fmaf(pb, inv[i16][1], l[t]);
+        pf[t][i16] = transpose8x8(split2(pa, pb));
+      }
+    }
+    // --- outputs
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int tok = i16 * 16 + 2 * c + (k & 1) + (k >> 1) * 8;
-          uint4 x = *reinterpret_cast<const uint4*>(vt + tok * D + ((g ^ (tok & 7)) << 4));
-          if (partial && !(seen >> tok & 1)) x = make_uint4(0, 0, 0, 0);  // may hold a NaN code: 0 x NaN
-          w[k][0] = x.x, w[k][1] = x.y, w[k][2] = x.z, w[k][3] = x.w;
-        }
+    for (int k = 0; k < 2; ++k) {
+      uint32_t keep[2] = {~0u, ~0u};
+      if (partial) {  // what is not seen may hold a NaN code, and 0 x NaN is NaN
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const uint32_t sel = (d & 1) ? 0x7362 : 0x5140;
-          const uint32_t x = __byte_perm(w[0][d >> 1], w[1][d >> 1], sel), y = __byte_perm(w[2][d >> 1], w[3][d >> 1], sel);
-          const uint32_t a0 = to_f16x2(x & 0xffffu), a1 = to_f16x2(x >> 16), a2 = to_f16x2(y & 0xffffu), a3 = to_f16x2(y >> 16);
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma_f16(acc[t][d], a0, a1, a2, a3, pf[t][i16][0], pf[t][i16][1]);
-        }
+          for (int e = 0; e < 4; ++e) {
+            const int x = 2 * c + (e >> 1), tok = k * 32 + half * 16 + ((e & 1) ? 8 + (x ^ 4) : x);
+            if (!(seen >> tok & 1)) keep[half] &= ~(0xffu << (8 * e));
+          }
+      }
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        uint32_t a[4];
+        ldsm_t(a, (ring_a + sv * TILE + k * 32 * D + v_off) ^ (d << 4));
+        if (partial) a[0] &= keep[0], a[1] &= keep[0], a[2] &= keep[1], a[3] &= keep[1];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma_e4m3(acc[t][d], a, pf[t][2 * k], pf[t][2 * k + 1]);
       }
     }
     __syncwarp();
@@ -558,33 +564,23 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
       const bool whole = ends && !begun_before;
       const long slot = (r * 2 + (begun_before ? 0 : 1)) * p.G;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        float sum = l[t];
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          float sum = l[t][cc];
+        for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const int h = 4 * t + c;
+        if (h >= p.G) continue;
+        const float rl = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+        bf16* dst = p.out + (((long)b * p.Hkv + hk) * p.G + h) * D + g;
+        float* part = p.part_o + (slot + h) * D + g;
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          const int h = t * 8 + 2 * c + cc;
-          if (h < p.G) {
-            if (whole) {
-              const float rl = sum == 0.f ? 0.f : 1.f / sum;
-              bf16* dst = p.out + (((long)b * p.Hkv + hk) * p.G + h) * D + 16 * g;
-              float f[8];
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                for (int d = 0; d < 4; ++d) f[2 * d] = acc[t][4 * half + d][cc] * rl, f[2 * d + 1] = acc[t][4 * half + d][2 + cc] * rl;
-                store8(dst + 8 * half, f);
-              }
-            } else {
-              float* dst = p.part_o + (slot + h) * D + 16 * g;
-#pragma unroll
-              for (int d = 0; d < 4; ++d)
-                *reinterpret_cast<float4*>(dst + 4 * d) = make_float4(acc[t][2 * d][cc], acc[t][2 * d][2 + cc], acc[t][2 * d + 1][cc], acc[t][2 * d + 1][2 + cc]);
-              if (g == 0) p.part_ml[slot + h] = make_float2(m[t][cc], sum);
-            }
-          }
+        for (int d = 0; d < 8; ++d) {
+          const float o0 = fmaf(acc[t][d][1], 0.03125f, acc[t][d][0]) * rl, o1 = fmaf(acc[t][d][3], 0.03125f, acc[t][d][2]) * rl;
+          if (whole) dst[16 * d] = __float2bfloat16(o0), dst[16 * d + 8] = __float2bfloat16(o1);
+          else part[16 * d] = o0, part[16 * d + 8] = o1;
         }
+        if (!whole && g == 0) p.part_ml[slot + h] = make_float2(m[t], sum);
+      }
       fresh = true;
       begun_before = false;
     }
@@ -762,7 +758,7 @@ at::Tensor paged_decode_attn_fp8(at::Tensor q, at::Tensor k, at::Tensor v, at::T
   const DecParams p{(const bf16*)q.data_ptr(), block_table.data_ptr<int>(), seq_lens.data_ptr<int>(), c.ks, c.vs, (bf16*)out.data_ptr(),
                     part_o.data_ptr<float>(), (float2*)part_ml.data_ptr<float>(), prefix.data_ptr<int>(), c.pages, (int)B, G, c.Hkv, c.P,
                     (int)block_table.size(1), box, (float)(scale * 1.4426950408889634)};
-  auto kern = G <= 8 ? decode_k<1> : decode_k<2>;
+  auto kern = G <= 4 ? decode_k<1> : G <= 8 ? decode_k<2> : decode_k<4>;
   smem_attr((const void*)kern, DEC_SMEM);
   launch_pdl(kern, dim3(grid), dim3(NW * 32), DEC_SMEM, stream(), tk, tv, p);
   AX_LAUNCH_OK();
