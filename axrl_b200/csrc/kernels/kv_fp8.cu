@@ -214,8 +214,8 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // Softmax in the log2 domain on w_t = scale log2(e) q.k_t + e_t, the exponent of V folded in: P_t = 2^{w_t - max w} <= 1
 // multiplies the codes themselves, and the normaliser is l = sum P_t 2^{-e_t} in fp32, unrounded.
 constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 3, TILE = UNIT * D;  // TILE: bytes of one slot
-constexpr int MAXB = 4096;
-constexpr int DEC_SMEM = 1024 + NW * SLOTS * TILE + NW * SLOTS * UNIT + NW * SLOTS * 8 + NW * SLOTS * 4 + (MAXB + 1) * 4;
+constexpr int MAXB = 2048;
+constexpr int DEC_SMEM = 1024 + NW * SLOTS * TILE + NW * SLOTS * UNIT + NW * SLOTS * 8 + NW * SLOTS * 4 + (2 * MAXB + 1) * 4;
 
 __device__ int g_decode_err;  // first wait that gave up (0: none)
 
@@ -227,7 +227,7 @@ struct DecParams {
   bf16* out;           // (B, Hq, 128)
   float* part_o;       // (ranges, 2, G, 128)
   float2* part_ml;     // (ranges, 2, G): max, sum
-  int* prefix;         // (B + 1): units of a kv head before sequence b, for merge_k
+  int* plan;           // (B + 3), for merge_k: units of a kv head before sequence b, then units of a range, ranges with one more
   long pages;
   int B, G, Hkv, P, max_pages, box;  // box: token rows of one TMA load, gcd(P, 64)
   float scale_log2;
@@ -242,9 +242,12 @@ __device__ __forceinline__ bool wait_tile(uint64_t* bar, uint32_t phase) {
     }
   return true;
 }
-__device__ __forceinline__ int dec_len(const DecParams& p, int b) { return (int)min((long)max(p.lens[b], 0), (long)p.max_pages * p.P); }
-// First unit of range r of n over W units; n <= W, so no range is empty.
-__device__ __forceinline__ long range_lo(long r, long W, long n) { return r * W / n; }
+// The W units fall into ranges of `base` units, the first `extra` of them one longer.
+struct Ranges {
+  int base, extra;
+  __device__ int lo(int r) const { return r * base + min(r, extra); }
+  __device__ int of(int x) const { return x < extra * (base + 1) ? x / (base + 1) : extra + (x - extra * (base + 1)) / base; }
+};
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -296,7 +299,8 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
   uint8_t* sc = reinterpret_cast<uint8_t*>(sm + NW * SLOTS * TILE) + warp * SLOTS * UNIT;  // scale bytes of a slot's tokens
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + NW * SLOTS * (TILE + UNIT)) + warp * SLOTS;
   int* meta = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 8)) + warp * SLOTS;  // chunks of a slot that were loaded
-  int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12));
+  int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12));  // units of the sequences before
+  int* s_len = prefix + MAXB + 1;
   __shared__ int s_warp[NW];
 
   if (lane == 0) {
@@ -305,12 +309,14 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
   }
   pdl_trigger();
   pdl_wait();
-  // exclusive prefix of the units of each sequence
   {
     const int per = (p.B + NW * 32 - 1) / (NW * 32), b0 = threadIdx.x * per;
     int sum = 0;
-    for (int i = 0; i < per; ++i)
-      if (b0 + i < p.B) sum += (dec_len(p, b0 + i) + UNIT - 1) / UNIT;
+    for (int i = b0; i < min(b0 + per, p.B); ++i) {
+      const int n = (int)min((long)max(p.lens[i], 0), (long)p.max_pages * p.P);
+      s_len[i] = n;
+      sum += (n + UNIT - 1) / UNIT;
+    }
     int x = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -320,27 +326,28 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
     int before = x - sum;
-    for (int w = 0; w < warp; ++w) before += s_warp[w];
-    for (int i = 0; i < per; ++i)
-      if (b0 + i < p.B) {
-        prefix[b0 + i] = before;
-        before += (dec_len(p, b0 + i) + UNIT - 1) / UNIT;
-      }
+#pragma unroll
+    for (int w = 0; w < NW; ++w) before += w < warp ? s_warp[w] : 0;
+    for (int i = b0; i < min(b0 + per, p.B); ++i) {
+      prefix[i] = before;
+      before += (s_len[i] + UNIT - 1) / UNIT;
+    }
     if (threadIdx.x == NW * 32 - 1) prefix[p.B] = before;
     __syncthreads();
-    if (blockIdx.x == 0)
-      for (int i = threadIdx.x; i <= p.B; i += NW * 32) p.prefix[i] = prefix[i];
   }
-  const long W = (long)prefix[p.B] * p.Hkv;
-  const long nr = min((long)gridDim.x * NW, W);
-  const long r = (long)warp * gridDim.x + blockIdx.x;  // neighbouring ranges on different SMs: few units still use every SM
+  const int W = prefix[p.B] * p.Hkv, nr = min((int)gridDim.x * NW, W);
+  const Ranges rg{W / max(nr, 1), W - W / max(nr, 1) * nr};
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i <= p.B; i += NW * 32) p.plan[i] = prefix[i];
+    if (threadIdx.x == 0) p.plan[p.B + 1] = rg.base, p.plan[p.B + 2] = rg.extra;
+  }
+  const int r = warp * gridDim.x + blockIdx.x;  // neighbouring ranges on different SMs: few units still use every SM
   if (r >= nr) return;
-  const long x0 = range_lo(r, W, nr);
-  const int n_units = (int)(range_lo(r + 1, W, nr) - x0);
+  const int x0 = rg.lo(r), n_units = rg.lo(r + 1) - x0;
 
   int b, hk, u, U, len;  // unit that is worked on next
   {
-    const int pos = (int)(x0 / p.Hkv);  // sequence b: prefix[b] <= pos < prefix[b + 1]
+    const int pos = x0 / p.Hkv;  // sequence b: prefix[b] <= pos < prefix[b + 1]
     int lo = 0, hi = p.B - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -349,9 +356,9 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     }
     b = lo;
     U = prefix[b + 1] - prefix[b];
-    const int rem = (int)(x0 - (long)prefix[b] * p.Hkv);
+    const int rem = x0 - prefix[b] * p.Hkv;
     hk = rem / U, u = rem % U;
-    len = dec_len(p, b);
+    len = s_len[b];
   }
   // lane `ch` < chunks loads the box of tokens [ch box, (ch + 1) box) of a unit
   const int chunks = UNIT / p.box;
@@ -375,7 +382,7 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     x.hk = 0;
     do ++x.b;
     while (x.b < p.B - 1 && prefix[x.b + 1] == prefix[x.b]);
-    if (x.b < p.B) x.U = prefix[x.b + 1] - prefix[x.b], x.len = dec_len(p, x.b);
+    if (x.b < p.B) x.U = prefix[x.b + 1] - prefix[x.b], x.len = s_len[x.b];
   };
   Loader ld{b, hk, u, U, len, n_units, (int)(((long)u * UNIT + lane * p.box) / p.P), (int)(((long)u * UNIT + lane * p.box) % p.P), -1};
   fetch_page(ld);
@@ -456,7 +463,7 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     if (!__all_sync(0xffffffffu, wait_tile(&full[sk], (j / SLOTS) & 1))) break;
     const int nval = min(UNIT, len - u * UNIT), loaded = meta[sk];
     const bool partial = nval < UNIT || __popc(loaded) < chunks;
-    float s[NT][4][2], kf[4][2];
+    float s[NT][4][2];
 #pragma unroll
     for (int i16 = 0; i16 < 4; ++i16) {
       float sa[NT][4];
@@ -469,10 +476,9 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
 #pragma unroll
         for (int t = 0; t < NT; ++t) mma_e4m3(sa[t], a, qf[t][2 * k], qf[t][2 * k + 1]);
       }
+      const float ka = scale_value(sc[sk * UNIT + i16 * 16 + tok_a]), kb = scale_value(sc[sk * UNIT + i16 * 16 + tok_b]);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s[t][i16][0] = fmaf(sa[t][1], 0.03125f, sa[t][0]), s[t][i16][1] = fmaf(sa[t][3], 0.03125f, sa[t][2]);
-      kf[i16][0] = scale_value(sc[sk * UNIT + i16 * 16 + tok_a]);
-      kf[i16][1] = scale_value(sc[sk * UNIT + i16 * 16 + tok_b]);
+      for (int t = 0; t < NT; ++t) s[t][i16][0] = fmaf(sa[t][1], 0.03125f, sa[t][0]) * ka, s[t][i16][1] = fmaf(sa[t][3], 0.03125f, sa[t][2]) * kb;
     }
     __syncwarp();
     load_next();
@@ -494,7 +500,7 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         const float e = byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(0x4b000000u + byte) - 8388735.f;  // byte - 127
         inv[i16][hh] = __uint_as_float((uint32_t)max((int)((254 - (int)byte) << 23), 0x400000));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][i16][hh] = fmaf(s[t][i16][hh], kf[i16][hh] * qs[t], e);
+        for (int t = 0; t < NT; ++t) s[t][i16][hh] = fmaf(s[t][i16][hh], qs[t], e);
       }
     if (partial) {
 #pragma unroll
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     const bool ends = u == U - 1;
     if (ends || i == n_units - 1) {
       const bool whole = ends && !begun_before;
-      const long slot = (r * 2 + (begun_before ? 0 : 1)) * p.G;
+      const int slot = (r * 2 + (begun_before ? 0 : 1)) * p.G;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float sum = l[t];
@@ -572,7 +578,7 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         if (h >= p.G) continue;
         const float rl = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
         bf16* dst = p.out + (((long)b * p.Hkv + hk) * p.G + h) * D + g;
-        float* part = p.part_o + (slot + h) * D + g;
+        float* part = p.part_o + (long)(slot + h) * D + g;
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
           const float o0 = fmaf(acc[t][d][1], 0.03125f, acc[t][d][0]) * rl, o1 = fmaf(acc[t][d][3], 0.03125f, acc[t][d][2]) * rl;
@@ -590,7 +596,7 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         hk = 0;
         do ++b;
         while (b < p.B - 1 && prefix[b + 1] == prefix[b]);
-        if (b < p.B) U = prefix[b + 1] - prefix[b], len = dec_len(p, b);
+        if (b < p.B) U = prefix[b + 1] - prefix[b], len = s_len[b];
       }
     }
   }
@@ -599,42 +605,72 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
 }
 
 // The pairs that more than one range holds: out = sum_r 2^{m_r - M} o_r / sum_r 2^{m_r - M} l_r; zeros for empty sequences.
-// One warp per (sequence, q head).
-__global__ void __launch_bounds__(128) merge_k(DecParams p, long ranges) {
+// One CTA per (sequence, kv head).  Its MW warps are dealt to the heads of the group and, where those are fewer, to
+// stripes of the partials, whose loads are all in flight at once (a long context has up to 2 x 74 of them on 16 pairs: one
+// warp walking them took 42 us, stripes 3).
+constexpr int MW = 8, MBATCH = 4;
+
+__global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
+  __shared__ float s_o[MW][D];
+  __shared__ float2 s_ml[MW];
   pdl_trigger();
   pdl_wait();
-  const long w = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31, Hq = p.Hkv * p.G;
-  if (w >= (long)p.B * Hq) return;
-  const int b = (int)(w / Hq), h = (int)(w % Hq), hk = h / p.G;
-  const long U = p.prefix[b + 1] - p.prefix[b];
-  float4 o = make_float4(0, 0, 0, 0);
-  if (U > 0) {
-    const long W = (long)p.prefix[p.B] * p.Hkv, nr = min(ranges, W);
-    const long x0 = (long)p.prefix[b] * p.Hkv + hk * U;
-    const long r0 = ((x0 + 1) * nr - 1) / W, r1 = ((x0 + U) * nr - 1) / W;  // ranges of its first and last unit
-    if (r0 == r1) return;  // finished by its warp
-    float M = -INFINITY;
-    const long first = (r0 * 2 + 1) * p.G + h % p.G;  // then (r * 2) * G + head
-    for (long r = r0 + lane; r <= r1; r += 32) M = fmaxf(M, p.part_ml[r == r0 ? first : r * 2 * p.G + h % p.G].x);
-    M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-#pragma unroll 4
-    for (long r = r0; r <= r1; ++r) {
-      const long i = r == r0 ? first : r * 2 * p.G + h % p.G;
-      const float2 ml = p.part_ml[i];
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + i * D + 4 * lane);
-      const float f = ex2(ml.x - ref);
-      L = fmaf(f, ml.y, L);
-      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+  const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = p.plan[b], U = p.plan[b + 1] - first;
+  const Ranges rg{p.plan[p.B + 1], p.plan[p.B + 2]};
+  bf16* out = p.out + ((long)b * p.Hkv + hk) * p.G * D;
+  if (U == 0) {
+    for (int i = threadIdx.x; i < p.G * D / 8; i += MW * 32) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int x0 = first * p.Hkv + hk * U, r0 = rg.of(x0), r1 = rg.of(x0 + U - 1);  // ranges of its first and last unit
+  if (r0 == r1) return;  // finished by its warp
+  const int stripes = p.G >= MW ? 1 : MW / p.G, stripe = warp / p.G;  // (a head and a stripe) per warp, heads in turn if G > MW
+  if (stripes == 1 && stripe > 0) return;
+  for (int h = warp % p.G; h < p.G; h += MW) {
+    float M = -INFINITY, L = 0.f;
+    float4 o = make_float4(0, 0, 0, 0);
+    if (stripe < stripes)
+      for (int r = r0 + stripe; r <= r1; r += stripes * MBATCH) {
+        float2 ml[MBATCH];
+        float4 v[MBATCH];
+        float mx = M;
+#pragma unroll
+        for (int k = 0; k < MBATCH; ++k) {
+          const int rk = r + k * stripes, i = (rk * 2 + (rk == r0 ? 1 : 0)) * p.G + h;  // the pair starts in its first range: slot 1
+          ml[k] = rk <= r1 ? p.part_ml[i] : make_float2(-INFINITY, 0.f);
+          v[k] = rk <= r1 ? *reinterpret_cast<const float4*>(p.part_o + (long)i * D + 4 * lane) : make_float4(0, 0, 0, 0);
+          mx = fmaxf(mx, ml[k].x);
+        }
+        const float ref = mx == -INFINITY ? 0.f : mx, a = ex2(M - ref);
+        M = mx;
+        L *= a, o.x *= a, o.y *= a, o.z *= a, o.w *= a;
+#pragma unroll
+        for (int k = 0; k < MBATCH; ++k) {
+          const float f = ex2(ml[k].x - ref);
+          L = fmaf(f, ml[k].y, L);
+          o.x = fmaf(f, v[k].x, o.x), o.y = fmaf(f, v[k].y, o.y), o.z = fmaf(f, v[k].z, o.z), o.w = fmaf(f, v[k].w, o.w);
+        }
+      }
+    if (stripes > 1) {
+      *reinterpret_cast<float4*>(&s_o[warp][4 * lane]) = o;
+      if (lane == 0) s_ml[warp] = make_float2(M, L);
+      __syncthreads();  // G < MW: every warp passes here once
+      if (stripe > 0) return;
+      for (int k = 1; k < stripes; ++k) {
+        const float2 ml = s_ml[warp + k * p.G];
+        const float4 v = *reinterpret_cast<const float4*>(&s_o[warp + k * p.G][4 * lane]);
+        const float mx = fmaxf(M, ml.x), ref = mx == -INFINITY ? 0.f : mx, a = ex2(M - ref), f = ex2(ml.x - ref);
+        M = mx;
+        L = fmaf(f, ml.y, L * a);
+        o.x = fmaf(f, v.x, o.x * a), o.y = fmaf(f, v.y, o.y * a), o.z = fmaf(f, v.z, o.z * a), o.w = fmaf(f, v.w, o.w * a);
+      }
     }
     const float rl = L == 0.f ? 0.f : 1.f / L;
-    o.x *= rl, o.y *= rl, o.z *= rl, o.w *= rl;
+    bf16* dst = out + h * D + 4 * lane;
+    *reinterpret_cast<bf162*>(dst) = __floats2bfloat162_rn(o.x * rl, o.y * rl);
+    *reinterpret_cast<bf162*>(dst + 2) = __floats2bfloat162_rn(o.z * rl, o.w * rl);
   }
-  bf16* dst = p.out + w * D + 4 * lane;
-  *reinterpret_cast<bf162*>(dst) = __floats2bfloat162_rn(o.x, o.y);
-  *reinterpret_cast<bf162*>(dst + 2) = __floats2bfloat162_rn(o.z, o.w);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -742,7 +778,7 @@ at::Tensor paged_decode_attn_fp8(at::Tensor q, at::Tensor k, at::Tensor v, at::T
   AX_CHECK(B <= MAXB, "decode batch must be <= ", MAXB);
   const long rows = c.pages * c.Hkv * c.P;
   AX_CHECK(rows < (1L << 31), "fp8 cache: pages * Hkv * page size must be below 2^31");
-  AX_CHECK(B * (block_table.size(1) * c.P / UNIT + 1) < (1L << 31), "block_table: too many tokens");
+  AX_CHECK(B * (block_table.size(1) * c.P / UNIT + 1) * c.Hkv < (1L << 31), "block_table: too many tokens");
   const c10::cuda::CUDAGuard guard(dev);
   auto out = at::empty_like(q);
   if (B == 0) return out;
@@ -751,18 +787,18 @@ at::Tensor paged_decode_attn_fp8(at::Tensor q, at::Tensor k, at::Tensor v, at::T
   const long ranges = (long)grid * NW;
   // freed after the launches, so the memory is handed on in stream order (and belongs to the graph when captured)
   auto part_o = at::empty({ranges * 2 * G * D}, q.options().dtype(at::kFloat)), part_ml = at::empty({ranges * 2 * G * 2}, part_o.options());
-  auto prefix = at::empty({B + 1}, q.options().dtype(at::kInt));
+  auto plan = at::empty({B + 3}, q.options().dtype(at::kInt));
   int box = 16;
   while (box < 64 && c.P % (2 * box) == 0) box *= 2;
   const CUtensorMap tk = codes_map(c.k, rows, box), tv = codes_map(c.v, rows, box);
   const DecParams p{(const bf16*)q.data_ptr(), block_table.data_ptr<int>(), seq_lens.data_ptr<int>(), c.ks, c.vs, (bf16*)out.data_ptr(),
-                    part_o.data_ptr<float>(), (float2*)part_ml.data_ptr<float>(), prefix.data_ptr<int>(), c.pages, (int)B, G, c.Hkv, c.P,
+                    part_o.data_ptr<float>(), (float2*)part_ml.data_ptr<float>(), plan.data_ptr<int>(), c.pages, (int)B, G, c.Hkv, c.P,
                     (int)block_table.size(1), box, (float)(scale * 1.4426950408889634)};
   auto kern = G <= 4 ? decode_k<1> : G <= 8 ? decode_k<2> : decode_k<4>;
   smem_attr((const void*)kern, DEC_SMEM);
   launch_pdl(kern, dim3(grid), dim3(NW * 32), DEC_SMEM, stream(), tk, tv, p);
   AX_LAUNCH_OK();
-  launch_pdl(merge_k, dim3((unsigned)((B * Hq + 3) / 4)), dim3(128), 0, stream(), p, ranges);
+  launch_pdl(merge_k, dim3((unsigned)(B * c.Hkv)), dim3(MW * 32), 0, stream(), p);
   AX_LAUNCH_OK();
   return out;
 }
