@@ -199,20 +199,21 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // others leave fp32 partials (at most two per warp), which merge_k combines.  A warp works alone: its own ring
 // of 8 KB slots (K and V tiles in turn) filled by its own TMA loads (128-byte swizzle), no barrier with other warps.
 //
-// Both products run on e4m3 operands as they lie in the cache (m16n8k32, fp32 sums), so no code is ever converted:
-//   S^T (tokens x columns) = Kc Q^T,   O^T (dims x columns) += Vc^T P^T   (ldmatrix transposes the V bytes)
-// The other factor is split into two e4m3 terms that take a column each: x = hi + lo / 32 with hi = e4m3(x) and
-// lo = e4m3(32 (x - hi)), both scaled so that hi fills e4m3's range.  A bf16 q has 8 significant bits and splits exactly
-// (but for what is below 2^-22 of the row's largest); P keeps 8 bits, the precision of a bf16 P (at most 2^-8 of each
-// probability, 2^-23 of the largest for small ones).  Eight columns are the hi and lo of four heads; groups of 5 to 16
-// heads take two or four column tiles.  With f16 operands instead, the conversions of the codes were 60 % of 1590
-// instructions a unit and bound the kernel (74.4 us for 64 sequences of 146k tokens, against 46 us of bytes).
-//
-// P^T is the transpose (movmatrix) of the S^T fragment: one register holds hi and lo of two tokens.  Rows of S^T map to
-// tokens so that these two lie 4 apart mod 8, which keeps both ldmatrix forms free of bank conflicts on swizzled tiles.
+// Both products are m16n8k16 with f16 operands and fp32 sums; f16 holds every e4m3 code exactly:
+//   S^T (tokens x heads) = Kc Q^T,   O^T (dims x heads) += Vc^T P^T
+// A lane gets four consecutive codes of a token row (ldmatrix) or of a column of V (its transposing byte form) in one
+// register: two conversions make them the two halves of an A fragment, because the contraction index may be permuted as
+// long as both operands agree.  P^T is the transpose (movmatrix) of the S^T fragment.  Rows of S^T map to tokens so
+// that each ldmatrix phase meets eight tokens that differ mod 8: no bank conflicts on swizzled tiles.  Up to eight heads of a
+// group fill the n = 8 columns; groups of 9 to 16 take two column tiles.  The e4m3 form of mma.sync needs no conversions in
+// the source but is no faster here: measured 5.4 clk per 16 x 32 step on an SM with two 8-bit terms per head, against 6.3
+// clk for the load, conversions and two products above, which serve twice the heads (256 short sequences with groups of
+// eight: 56.5 us against TODO).
 //
 // Softmax in the log2 domain on w_t = scale log2(e) q.k_t + e_t, the exponent of V folded in: P_t = 2^{w_t - max w} <= 1
-// multiplies the codes themselves, and the normaliser is l = sum P_t 2^{-e_t} in fp32, unrounded.
+// rounds to f16 (2^-11, finer than bf16) and multiplies the codes themselves, and the normaliser is l = sum P_t 2^{-e_t}
+// in fp32, unrounded.  Whatever falls below f16 is 2^-24 of the largest weighted term.  q rows are scaled by a power of
+// two so that their largest is in [2^14, 2^15) and round to f16 exactly but for what is below 2^-28 of it.
 constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 3, TILE = UNIT * D;  // TILE: bytes of one slot
 constexpr int MAXB = 2048;
 constexpr int DEC_SMEM = 1024 + NW * SLOTS * TILE + NW * SLOTS * UNIT + NW * SLOTS * 8 + NW * SLOTS * 4 + (2 * MAXB + 1) * 4;
@@ -249,9 +250,10 @@ struct Ranges {
   __device__ int of(int x) const { return x < extra * (base + 1) ? x / (base + 1) : extra + (x - extra * (base + 1)) / base; }
 };
 
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// Not volatile: the products may move behind later ldmatrix loads, which keep their order.
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Four 8 x 16-byte matrices: the A fragment of 16 rows x 32 bytes.
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -261,15 +263,17 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
-// x, y (|.| <= 256) as e4m3 pairs: hi in the low half, 32 times the remainder in the high half.
-__device__ __forceinline__ uint32_t split2(float x, float y) {
-  const uint32_t hi = to_e4m3x2(x, y);
-  const float2 h = from_e4m3x2(hi);
-  return hi | to_e4m3x2(fmaf(h.x, -32.f, 32.f * x), fmaf(h.y, -32.f, 32.f * y)) << 16;
+// Four codes as two pairs of halves.
+__device__ __forceinline__ void halves(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{.reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -298,14 +302,18 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
   char* ring = sm + warp * SLOTS * TILE;
   uint8_t* sc = reinterpret_cast<uint8_t*>(sm + NW * SLOTS * TILE) + warp * SLOTS * UNIT;  // scale bytes of a slot's tokens
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + NW * SLOTS * (TILE + UNIT)) + warp * SLOTS;
-  int* meta = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 8)) + warp * SLOTS;  // chunks of a slot that were loaded
+  uchar4* meta = reinterpret_cast<uchar4*>(sm + NW * SLOTS * (TILE + UNIT + 8)) + warp * SLOTS;  // which chunks of a slot were loaded
   int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12));  // units of the sequences before
   int* s_len = prefix + MAXB + 1;
   __shared__ int s_warp[NW];
 
   if (lane == 0) {
-    for (int s = 0; s < SLOTS; ++s) tc::mbar_init(&full[s], 1);
+    for (int s = 0; s < SLOTS; ++s) tc::mbar_init(&full[s], UNIT / p.box);  // every loading lane arrives
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
   }
   pdl_trigger();
   pdl_wait();
@@ -348,11 +356,12 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
   int b, hk, u, U, len;  // unit that is worked on next
   {
     const int pos = x0 / p.Hkv;  // sequence b: prefix[b] <= pos < prefix[b + 1]
-    int lo = 0, hi = p.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] <= pos) lo = mid;
-      else hi = mid - 1;
+    int lo = 0, n = p.B;  // b in [lo, lo + n)
+    while (n > 1) {
+      const int step = (n + 31) >> 5, at = lo + lane * step;
+      const int k = 31 - __clz(__ballot_sync(0xffffffffu, at < lo + n && prefix[min(at, p.B)] <= pos));
+      n = min(step, lo + n - (lo + k * step));
+      lo += k * step;
     }
     b = lo;
     U = prefix[b + 1] - prefix[b];
@@ -397,19 +406,16 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
       }
     }
     const int s = nj % SLOTS;
-    const uint32_t ok = __ballot_sync(0xffffffffu, row >= 0);
-    if (lane == 0) {
-      meta[s] = (int)ok;
-      tc::mbar_expect_tx(&full[s], __popc(ok) * p.box * (D + 1));
-    }
-    __syncwarp();
-    if (row >= 0) {
-      tc::tma_2d(ring + s * TILE + lane * p.box * D, (nj & 1) ? &tv : &tk, 0, row, &full[s]);
-      bulk_bytes(sc + s * UNIT + lane * p.box, ((nj & 1) ? p.vs : p.ks) + row, p.box, &full[s]);
+    if (loads) {
+      reinterpret_cast<uint8_t*>(&meta[s])[lane] = row >= 0;
+      tc::mbar_expect_tx(&full[s], row >= 0 ? p.box * (D + 1) : 0);
+      if (row >= 0) {
+        tc::tma_2d(ring + s * TILE + lane * p.box * D, (nj & 1) ? &tv : &tk, 0, row, &full[s]);
+        bulk_bytes(sc + s * UNIT + lane * p.box, ((nj & 1) ? p.vs : p.ks) + row, p.box, &full[s]);
+      }
     }
     ++nj;
   };
-  __syncwarp();
   for (int i = 0; i < SLOTS; ++i) load_next();
 
   // row x of S^T is token x, row 8 + x token 8 + (x ^ 4) of 16
@@ -419,20 +425,20 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     const int x = lane & 7, tok = (lane >> 3 & 1) ? 8 + (x ^ 4) : x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) k_off[i] = tok * D + (((2 * i + (lane >> 4)) ^ (tok & 7)) << 4);
-    const int y = lane >> 1 & 7, tv16 = (lane & 1) ? 8 + (y ^ 4) : y;  // rows of V in the order of P's bytes
+    const int y = (lane >> 1 & 6) + (lane & 1), tv16 = (lane >> 1 & 1) ? 8 + (y ^ 4) : y;  // rows of V in the order of P's fragment
     v_off = ((lane >> 4) * 16 + tv16) * D + ((tv16 & 7) << 4);
   }
   const uint32_t ring_a = tc::s32(ring);
-  float acc[NT][8][4], m[NT], l[NT], qs[NT];
-  uint32_t qf[NT][8];
+  float acc[NT][8][4], m[NT][2], l[NT][2], qs[NT][2];  // columns 2c, 2c + 1 of a tile: heads 8 t + 2 c, + 1
+  uint32_t qf[NT][16];
   bool fresh = true, begun_before = u > 0;  // the pair at the start of the range may have begun in an earlier one
   int j = 0;
   for (int i = 0; i < n_units; ++i) {
-    if (fresh) {  // q columns of this pair: column g is hi (even) or lo (odd) of head 4 t + g / 2
+    if (fresh) {  // q columns of this pair: column g is head 8 t + g
       fresh = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int h = 4 * t + (g >> 1);
+        const int h = 8 * t + g;
         uint2 w[8];
         uint32_t top = 0;
 #pragma unroll
@@ -442,18 +448,18 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // largest value to [128, 256); rows that are not finite poison their scores through the factor
+        // 2^(141 - ex) takes the largest to [2^14, 2^15); a row that is not finite poisons its scores through the factor
         const uint32_t ex = top >> 23;
-        const float down = ex < 8u ? 1.f : __uint_as_float((261u - min(ex, 254u)) << 23);
-        const float up = ex == 255u ? __uint_as_float(0x7fffffffu) : p.scale_log2 * (ex < 8u ? 1.f : __uint_as_float((ex - 7u) << 23));
-        qs[t] = __shfl_sync(0xffffffffu, up, 8 * c);  // head 4 t + c
+        const float down = ex < 15u ? 1.f : __uint_as_float((268u - min(ex, 254u)) << 23);
+        const float up = ex == 255u ? __uint_as_float(0x7fffffffu) : p.scale_log2 * (ex < 15u ? 1.f : __uint_as_float((ex - 14u) << 23));
+        qs[t][0] = __shfl_sync(0xffffffffu, up, 8 * c);  // column 2c
+        qs[t][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const uint32_t x = split2(__uint_as_float(w[k].x << 16) * down, __uint_as_float(w[k].x & 0xffff0000u) * down);
-          const uint32_t y = split2(__uint_as_float(w[k].y << 16) * down, __uint_as_float(w[k].y & 0xffff0000u) * down);
-          qf[t][k] = __byte_perm(x, y, (g & 1) ? 0x7632 : 0x5410);
+          qf[t][2 * k] = pack_f16(__uint_as_float(w[k].x << 16) * down, __uint_as_float(w[k].x & 0xffff0000u) * down);
+          qf[t][2 * k + 1] = pack_f16(__uint_as_float(w[k].y << 16) * down, __uint_as_float(w[k].y & 0xffff0000u) * down);
         }
-        m[t] = -INFINITY, l[t] = 0.f;
+        m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) acc[t][d][0] = acc[t][d][1] = acc[t][d][2] = acc[t][d][3] = 0.f;
       }
@@ -461,28 +467,34 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     const int sk = j % SLOTS, sv = (j + 1) % SLOTS;
     // --- scores of 64 tokens
     if (!__all_sync(0xffffffffu, wait_tile(&full[sk], (j / SLOTS) & 1))) break;
-    const int nval = min(UNIT, len - u * UNIT), loaded = meta[sk];
+    const int nval = min(UNIT, len - u * UNIT);
+    const uchar4 ld4 = meta[sk];
+    const int loaded = ld4.x | (ld4.y & (chunks > 1)) << 1 | (chunks > 2 ? ld4.z << 2 | ld4.w << 3 : 0);
     const bool partial = nval < UNIT || __popc(loaded) < chunks;
-    float s[NT][4][2];
+    float s[NT][4][4];  // tokens tok_a, tok_b of 16 x the two columns
 #pragma unroll
     for (int i16 = 0; i16 < 4; ++i16) {
-      float sa[NT][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) sa[t][0] = sa[t][1] = sa[t][2] = sa[t][3] = 0.f;
+      for (int t = 0; t < NT; ++t) s[t][i16][0] = s[t][i16][1] = s[t][i16][2] = s[t][i16][3] = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        uint32_t a[4];
+        uint32_t a[4], x[8];
         ldsm4(a, ring_a + sk * TILE + i16 * 16 * D + k_off[k]);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma_e4m3(sa[t], a, qf[t][2 * k], qf[t][2 * k + 1]);
+        for (int e = 0; e < 4; ++e) halves(a[e], x[2 * e], x[2 * e + 1]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          mma_f16(s[t][i16], x[0], x[2], x[1], x[3], qf[t][4 * k], qf[t][4 * k + 1]);
+          mma_f16(s[t][i16], x[4], x[6], x[5], x[7], qf[t][4 * k + 2], qf[t][4 * k + 3]);
+        }
       }
       const float ka = scale_value(sc[sk * UNIT + i16 * 16 + tok_a]), kb = scale_value(sc[sk * UNIT + i16 * 16 + tok_b]);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s[t][i16][0] = fmaf(sa[t][1], 0.03125f, sa[t][0]) * ka, s[t][i16][1] = fmaf(sa[t][3], 0.03125f, sa[t][2]) * kb;
+      for (int t = 0; t < NT; ++t) s[t][i16][0] *= ka, s[t][i16][1] *= ka, s[t][i16][2] *= kb, s[t][i16][3] *= kb;
     }
     __syncwarp();
     load_next();
-    // --- w = scale log2(e) q.k + e, and 256 P = 2^{w - max w + 8}
+    // --- w = scale log2(e) q.k + e, and P = 2^{w - max w}
     if (!__all_sync(0xffffffffu, wait_tile(&full[sv], ((j + 1) / SLOTS) & 1))) break;
     uint64_t seen = ~0ull;  // tokens of the unit that count
     if (partial) {
@@ -500,7 +512,9 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         const float e = byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(0x4b000000u + byte) - 8388735.f;  // byte - 127
         inv[i16][hh] = __uint_as_float((uint32_t)max((int)((254 - (int)byte) << 23), 0x400000));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][i16][hh] = fmaf(s[t][i16][hh], qs[t], e);
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) s[t][i16][2 * hh + cc] = fmaf(s[t][i16][2 * hh + cc], qs[t][cc], e);
       }
     if (partial) {
 #pragma unroll
@@ -509,35 +523,39 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         for (int hh = 0; hh < 2; ++hh)
           if (!(seen >> (i16 * 16 + (hh ? tok_b : tok_a)) & 1)) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) s[t][i16][hh] = -INFINITY;
+            for (int t = 0; t < NT; ++t) s[t][i16][2 * hh] = s[t][i16][2 * hh + 1] = -INFINITY;
           }
     }
-    uint32_t pf[NT][4];
+    uint32_t pf[NT][4][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      float mx = fmaxf(s[t][0][0], s[t][0][1]);
+      float alpha[2], ref[2];
 #pragma unroll
-      for (int i16 = 1; i16 < 4; ++i16) mx = fmaxf(mx, fmaxf(s[t][i16][0], s[t][i16][1]));
+      for (int cc = 0; cc < 2; ++cc) {
+        float mx = fmaxf(s[t][0][cc], s[t][0][2 + cc]);
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      mx = fmaxf(m[t], mx);
-      const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen yet
-      const float alpha = ex2(m[t] - ref);
-      m[t] = mx;
-      l[t] *= alpha;
-      if (__any_sync(0xffffffffu, alpha != 1.f)) {
-        // accumulator columns 2c, 2c + 1 are hi and lo of this lane's head
+        for (int i16 = 1; i16 < 4; ++i16) mx = fmaxf(mx, fmaxf(s[t][i16][cc], s[t][i16][2 + cc]));
 #pragma unroll
-        for (int d = 0; d < 8; ++d) acc[t][d][0] *= alpha, acc[t][d][1] *= alpha, acc[t][d][2] *= alpha, acc[t][d][3] *= alpha;
+        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        mx = fmaxf(m[t][cc], mx);
+        ref[cc] = mx == -INFINITY ? 0.f : mx;  // nothing seen yet
+        alpha[cc] = ex2(m[t][cc] - ref[cc]);
+        m[t][cc] = mx;
+        l[t][cc] *= alpha[cc];
       }
-      const float shift = 8.f - ref;
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-      for (int i16 = 0; i16 < 4; ++i16) {
-        const float pa = ex2(s[t][i16][0] + shift), pb = ex2(s[t][i16][1] + shift);
-        l[t] = fmaf(pa, inv[i16][0], l[t]);
-        l[t] = fmaf(pb, inv[i16][1], l[t]);
-        pf[t][i16] = transpose8x8(split2(pa, pb));
+        for (int d = 0; d < 8; ++d) acc[t][d][0] *= alpha[0], acc[t][d][1] *= alpha[1], acc[t][d][2] *= alpha[0], acc[t][d][3] *= alpha[1];
       }
+#pragma unroll
+      for (int i16 = 0; i16 < 4; ++i16)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const float p0 = ex2(s[t][i16][2 * hh] - ref[0]), p1 = ex2(s[t][i16][2 * hh + 1] - ref[1]);
+          l[t][0] = fmaf(p0, inv[i16][hh], l[t][0]);
+          l[t][1] = fmaf(p1, inv[i16][hh], l[t][1]);
+          pf[t][i16][hh] = transpose8x8(pack_f16(p0, p1));
+        }
     }
     // --- outputs
 #pragma unroll
@@ -548,17 +566,22 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int x = 2 * c + (e >> 1), tok = k * 32 + half * 16 + ((e & 1) ? 8 + (x ^ 4) : x);
+            const int x = 2 * c + (e & 1), tok = k * 32 + half * 16 + (e >> 1 ? 8 + (x ^ 4) : x);
             if (!(seen >> tok & 1)) keep[half] &= ~(0xffu << (8 * e));
           }
       }
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
-        uint32_t a[4];
+        uint32_t a[4], x[8];
         ldsm_t(a, (ring_a + sv * TILE + k * 32 * D + v_off) ^ (d << 4));
         if (partial) a[0] &= keep[0], a[1] &= keep[0], a[2] &= keep[1], a[3] &= keep[1];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma_e4m3(acc[t][d], a, pf[t][2 * k], pf[t][2 * k + 1]);
+        for (int e = 0; e < 4; ++e) halves(a[e], x[2 * e], x[2 * e + 1]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          mma_f16(acc[t][d], x[0], x[2], x[1], x[3], pf[t][2 * k][0], pf[t][2 * k][1]);
+          mma_f16(acc[t][d], x[4], x[6], x[5], x[7], pf[t][2 * k + 1][0], pf[t][2 * k + 1][1]);
+        }
       }
     }
     __syncwarp();
@@ -570,23 +593,25 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
       const bool whole = ends && !begun_before;
       const int slot = (r * 2 + (begun_before ? 0 : 1)) * p.G;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float sum = l[t];
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const int h = 4 * t + c;
-        if (h >= p.G) continue;
-        const float rl = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
-        bf16* dst = p.out + (((long)b * p.Hkv + hk) * p.G + h) * D + g;
-        float* part = p.part_o + (long)(slot + h) * D + g;
+        for (int cc = 0; cc < 2; ++cc) {
+          float sum = l[t][cc];
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const float o0 = fmaf(acc[t][d][1], 0.03125f, acc[t][d][0]) * rl, o1 = fmaf(acc[t][d][3], 0.03125f, acc[t][d][2]) * rl;
-          if (whole) dst[16 * d] = __float2bfloat16(o0), dst[16 * d + 8] = __float2bfloat16(o1);
-          else part[16 * d] = o0, part[16 * d + 8] = o1;
+          for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          const int h = 8 * t + 2 * c + cc;
+          if (h < p.G) {
+            const float rl = sum == 0.f ? 0.f : 1.f / sum;
+            bf16* dst = p.out + (((long)b * p.Hkv + hk) * p.G + h) * D + g;
+            float* part = p.part_o + (long)(slot + h) * D + g;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+              if (whole) dst[16 * d] = __float2bfloat16(acc[t][d][cc] * rl), dst[16 * d + 8] = __float2bfloat16(acc[t][d][2 + cc] * rl);
+              else part[16 * d] = acc[t][d][cc], part[16 * d + 8] = acc[t][d][2 + cc];
+            }
+            if (!whole && g == 0) p.part_ml[slot + h] = make_float2(m[t][cc], sum);
+          }
         }
-        if (!whole && g == 0) p.part_ml[slot + h] = make_float2(m[t], sum);
-      }
       fresh = true;
       begun_before = false;
     }
@@ -794,7 +819,7 @@ at::Tensor paged_decode_attn_fp8(at::Tensor q, at::Tensor k, at::Tensor v, at::T
   const DecParams p{(const bf16*)q.data_ptr(), block_table.data_ptr<int>(), seq_lens.data_ptr<int>(), c.ks, c.vs, (bf16*)out.data_ptr(),
                     part_o.data_ptr<float>(), (float2*)part_ml.data_ptr<float>(), plan.data_ptr<int>(), c.pages, (int)B, G, c.Hkv, c.P,
                     (int)block_table.size(1), box, (float)(scale * 1.4426950408889634)};
-  auto kern = G <= 4 ? decode_k<1> : G <= 8 ? decode_k<2> : decode_k<4>;
+  auto kern = G <= 8 ? decode_k<1> : decode_k<2>;
   smem_attr((const void*)kern, DEC_SMEM);
   launch_pdl(kern, dim3(grid), dim3(NW * 32), DEC_SMEM, stream(), tk, tv, p);
   AX_LAUNCH_OK();

@@ -201,9 +201,8 @@ def test_gather(dev, T, hkv, P):
 # ----------------------------------------------------------------------------- decode
 def _exact_decode(q, cache, bt, lens, scale):
     """o in 64 bits and its tolerance.  A score is off by at most 2^-18 sum|q k| scale (32-bit sums of 128 products) and
-    2^-22 max|q| sum|k| scale (what the two 8-bit terms of q drop).  A probability held as two e4m3 terms is off by at
-    most 2^-4 x 2^-4 = 2^-8 of its value, and a small one by 2^-10 / 32 / 256 = 2^-23 of the largest weight.  The output
-    is rounded to bf16."""
+    2^-28 max|q| sum|k| scale (what q drops in 16 bits).  A probability is rounded to 16 bits, at most 2^-11 of its value
+    (2^-10 leaves room for its exponential), and a small one by 2^-24 of the largest weight.  The output is rounded to bf16."""
     B, Hq, _ = q.shape
     pages, Hkv, P, _ = cache.k.shape
     G = Hq // Hkv
@@ -220,10 +219,10 @@ def _exact_decode(q, cache, bt, lens, scale):
             qq = q[b, h * G:(h + 1) * G].double()
             p = torch.softmax(qq @ k.t() * scale, -1)
             off = 2.0 ** -18 * (qq.abs() @ k.abs().t() * abs(scale)).amax(-1, keepdim=True)
-            off = off + 2.0 ** -22 * qq.abs().amax(-1, keepdim=True) * k.abs().sum(-1).amax() * abs(scale)
+            off = off + 2.0 ** -28 * qq.abs().amax(-1, keepdim=True) * k.abs().sum(-1).amax() * abs(scale)
             a = p @ v.abs()
             o[b, h * G:(h + 1) * G] = p @ v
-            tol[b, h * G:(h + 1) * G] = 2.0 ** -8 * (p @ v).abs() + a * (2.0 ** -8 + 2 * off) + 2.0 ** -23 * slots.numel() * a.amax(-1, keepdim=True)
+            tol[b, h * G:(h + 1) * G] = 2.0 ** -8 * (p @ v).abs() + a * (2.0 ** -10 + 2 * off) + 2.0 ** -24 * slots.numel() * a.amax(-1, keepdim=True)
     return o, tol
 
 
