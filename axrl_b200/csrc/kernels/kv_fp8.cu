@@ -214,9 +214,10 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // rounds to f16 (2^-11, finer than bf16) and multiplies the codes themselves, and the normaliser is l = sum P_t 2^{-e_t}
 // in fp32, unrounded.  Whatever falls below f16 is 2^-24 of the largest weighted term.  q rows are scaled by a power of
 // two so that their largest is in [2^14, 2^15) and round to f16 exactly but for what is below 2^-28 of it.
-constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 3, TILE = UNIT * D;  // TILE: bytes of one slot
+constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 2, TILE = UNIT * D;  // TILE: bytes of one slot
 constexpr int MAXB = 2048;
-constexpr int DEC_SMEM = 1024 + NW * SLOTS * TILE + NW * SLOTS * UNIT + NW * SLOTS * 8 + NW * SLOTS * 4 + (2 * MAXB + 1) * 4;
+constexpr int Q_BYTES = MAXG * D * 2;  // q rows of a pair
+constexpr int DEC_SMEM = 1024 + NW * SLOTS * (TILE + UNIT + 8 + 4) + NW * Q_BYTES + (2 * MAXB + 1) * 4;
 
 __device__ int g_decode_err;  // first wait that gave up (0: none)
 
@@ -303,7 +304,8 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
   uint8_t* sc = reinterpret_cast<uint8_t*>(sm + NW * SLOTS * TILE) + warp * SLOTS * UNIT;  // scale bytes of a slot's tokens
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + NW * SLOTS * (TILE + UNIT)) + warp * SLOTS;
   uchar4* meta = reinterpret_cast<uchar4*>(sm + NW * SLOTS * (TILE + UNIT + 8)) + warp * SLOTS;  // which chunks of a slot were loaded
-  int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12));  // units of the sequences before
+  char* sq = sm + NW * SLOTS * (TILE + UNIT + 12) + warp * Q_BYTES;  // q rows of the pair that is loaded next
+  int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12) + NW * Q_BYTES);  // units of the sequences before
   int* s_len = prefix + MAXB + 1;
   __shared__ int s_warp[NW];
 
@@ -343,7 +345,9 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     if (threadIdx.x == NW * 32 - 1) prefix[p.B] = before;
     __syncthreads();
   }
-  const int W = prefix[p.B] * p.Hkv, nr = min((int)gridDim.x * NW, W);
+  // as few ranges as the longest one allows, so that nearly all have its length: the last units of a few longer ranges would
+  // run alone (two contexts of 100k: 20 units a warp and 21 for 35 of 1184 cost 3 of 72 us)
+  const int W = prefix[p.B] * p.Hkv, top = (W + gridDim.x * NW - 1) / (gridDim.x * NW), nr = W > 0 ? (W + top - 1) / top : 0;
   const Ranges rg{W / max(nr, 1), W - W / max(nr, 1) * nr};
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i <= p.B; i += NW * 32) p.plan[i] = prefix[i];
@@ -395,13 +399,20 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
   };
   Loader ld{b, hk, u, U, len, n_units, (int)(((long)u * UNIT + lane * p.box) / p.P), (int)(((long)u * UNIT + lane * p.box) % p.P), -1};
   fetch_page(ld);
-  int nj = 0, row = -1;  // next tile to load (even: K, odd: V of the same unit), its cache row
+  int nj = 0, row = -1;     // next tile to load (even: K, odd: V of the same unit), its cache row
+  bool new_pair = true;     // of `ld`: its q rows come with its K tile
   auto load_next = [&] {
     if ((nj & 1) == 0) {
       if (ld.left == 0) return;
+      if (new_pair && lane == 0) {
+        const int bytes = p.G * D * 2;
+        tc::mbar_tx(&full[nj % SLOTS], bytes);  // counted before the arrival below completes the phase
+        bulk_bytes(sq, p.q + ((long)ld.b * p.Hkv + ld.hk) * p.G * D, bytes, &full[nj % SLOTS]);
+      }
       row = ld.page >= 0 ? (int)(((long)ld.page * p.Hkv + ld.hk) * p.P) + ld.off : -1;
       if (--ld.left > 0) {
         next_unit(ld);
+        new_pair = ld.u == 0;
         fetch_page(ld);
       }
     }
@@ -434,6 +445,9 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
   bool fresh = true, begun_before = u > 0;  // the pair at the start of the range may have begun in an earlier one
   int j = 0;
   for (int i = 0; i < n_units; ++i) {
+    const int sk = j % SLOTS, sv = (j + 1) % SLOTS;
+    // --- scores of 64 tokens
+    if (!__all_sync(0xffffffffu, wait_tile(&full[sk], (j / SLOTS) & 1))) break;
     if (fresh) {  // q columns of this pair: column g is head 8 t + g
       fresh = false;
 #pragma unroll
@@ -443,7 +457,7 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         uint32_t top = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          w[k] = h < p.G ? *reinterpret_cast<const uint2*>(p.q + (((long)b * p.Hkv + hk) * p.G + h) * D + 16 * k + 4 * c) : make_uint2(0, 0);
+          w[k] = h < p.G ? *reinterpret_cast<const uint2*>(sq + h * D * 2 + 32 * k + 8 * c) : make_uint2(0, 0);
           top = max(top, max(max((w[k].x << 16) & 0x7fffffffu, w[k].x & 0x7fff0000u), max((w[k].y << 16) & 0x7fffffffu, w[k].y & 0x7fff0000u)));
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -464,20 +478,19 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
         for (int d = 0; d < 8; ++d) acc[t][d][0] = acc[t][d][1] = acc[t][d][2] = acc[t][d][3] = 0.f;
       }
     }
-    const int sk = j % SLOTS, sv = (j + 1) % SLOTS;
-    // --- scores of 64 tokens
-    if (!__all_sync(0xffffffffu, wait_tile(&full[sk], (j / SLOTS) & 1))) break;
     const int nval = min(UNIT, len - u * UNIT);
     const uchar4 ld4 = meta[sk];
     const int loaded = ld4.x | (ld4.y & (chunks > 1)) << 1 | (chunks > 2 ? ld4.z << 2 | ld4.w << 3 : 0);
     const bool partial = nval < UNIT || __popc(loaded) < chunks;
     float s[NT][4][4];  // tokens tok_a, tok_b of 16 x the two columns
 #pragma unroll
-    for (int i16 = 0; i16 < 4; ++i16) {
+    for (int i16 = 0; i16 < 4; ++i16)
 #pragma unroll
       for (int t = 0; t < NT; ++t) s[t][i16][0] = s[t][i16][1] = s[t][i16][2] = s[t][i16][3] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i16 = 0; i16 < 4; ++i16) {  // innermost: the four tiles' sums do not depend on each other
         uint32_t a[4], x[8];
         ldsm4(a, ring_a + sk * TILE + i16 * 16 * D + k_off[k]);
 #pragma unroll
@@ -488,6 +501,8 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
           mma_f16(s[t][i16], x[4], x[6], x[5], x[7], qf[t][4 * k + 2], qf[t][4 * k + 3]);
         }
       }
+#pragma unroll
+    for (int i16 = 0; i16 < 4; ++i16) {
       const float ka = scale_value(sc[sk * UNIT + i16 * 16 + tok_a]), kb = scale_value(sc[sk * UNIT + i16 * 16 + tok_b]);
 #pragma unroll
       for (int t = 0; t < NT; ++t) s[t][i16][0] *= ka, s[t][i16][1] *= ka, s[t][i16][2] *= kb, s[t][i16][3] *= kb;
