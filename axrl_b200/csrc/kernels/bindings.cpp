@@ -111,12 +111,14 @@ at::Tensor tc_linear_dgrad(at::Tensor dy, at::Tensor w);
 void adamw_p2p_step(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v, at::Tensor ptrs, int64_t s0, int64_t decay_end, double lr,
                     double b1, double b2, double eps, double wd, int64_t step, at::Tensor sqnorm, double clip, double extra_scale);
 void tc_linear_wgrad_acc(at::Tensor dy, at::Tensor x, at::Tensor acc, bool accumulate);
-std::vector<at::Tensor> qknorm_rope_cache_fp8(at::Tensor qkv, at::Tensor qw, at::Tensor kw, at::Tensor pos, at::Tensor inv_freq, int64_t nq,
-                                              int64_t nkv, double eps, at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor slots,
-                                              bool want_kv);
-void gather_kv_fp8(at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor slots, at::Tensor ko, at::Tensor vo);
-at::Tensor paged_decode_attn_fp8(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor block_table, at::Tensor seq_lens,
-                                 double scale);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qknorm_rope_cache_fp8(const at::Tensor& qkv, const at::Tensor& qw, const at::Tensor& kw,
+                                                                     const at::Tensor& pos, const at::Tensor& inv_freq, int64_t nq, int64_t nkv,
+                                                                     double eps, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
+                                                                     const at::Tensor& vs, const at::Tensor& slots, bool want_kv);
+std::tuple<at::Tensor, at::Tensor> gather_kv_fp8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
+                                                 const at::Tensor& slots, const c10::optional<at::Tensor>& out_k, const c10::optional<at::Tensor>& out_v);
+at::Tensor paged_decode_attn_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
+                                 const at::Tensor& block_table, const at::Tensor& seq_lens, double scale);
 int64_t kv_fp8_error();
 }  // namespace ax
 

@@ -7,6 +7,7 @@
 // code * scale is exact in bf16, so every reader sees the same values.  No counterpart in the reference
 // beyond its rollout engine's kv_cache_dtype option (axrl/configs.py RolloutWorkerConfig).
 #include <ATen/ops/zero.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda.h>
 
@@ -161,6 +162,8 @@ __global__ void __launch_bounds__(256) append_k(const bf16* __restrict__ qkv, co
 // ----------------------------------------------------------------------------- load
 // Rows of the cache as bf16: one thread per 16 codes of K or V; exact.
 __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict__ slots, bf16* __restrict__ ko, bf16* __restrict__ vo, long T) {
+  pdl_trigger();
+  pdl_wait();
   const long n = T * c.Hkv * 16;  // 8 chunks of 16 codes for K, then for V
   for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) {
     const int ch = (int)(i & 7), isv = (int)(i >> 3) & 1;
@@ -229,7 +232,7 @@ struct DecParams {
   bf16* out;           // (B, Hq, 128)
   float* part_o;       // (ranges, 2, G, 128)
   float2* part_ml;     // (ranges, 2, G): max, sum
-  int* plan;           // (B + 3), for merge_k: units of a kv head before sequence b, then units of a range, ranges with one more
+  int ranges;          // most ranges: warps of decode_k
   long pages;
   int B, G, Hkv, P, max_pages, box;  // box: token rows of one TMA load, gcd(P, 64)
   float scale_log2;
@@ -244,12 +247,24 @@ __device__ __forceinline__ bool wait_tile(uint64_t* bar, uint32_t phase) {
     }
   return true;
 }
-// The W units fall into ranges of `base` units, the first `extra` of them one longer.
+// W units in n ranges of `base` units, the first `extra` of them one longer.  As few ranges as the longest one allows, so
+// that nearly all have its length: the last units of a few longer ranges would run alone (two contexts of 100k: 20 units a
+// warp and 21 for 35 of 1184 cost 2 of 72 us).
 struct Ranges {
-  int base, extra;
+  int n, base, extra;
+  __device__ Ranges(int W, int most) {
+    const int top = max((W + most - 1) / most, 1);
+    n = (W + top - 1) / top;
+    base = W / max(n, 1);
+    extra = W - base * n;
+  }
   __device__ int lo(int r) const { return r * base + min(r, extra); }
   __device__ int of(int x) const { return x < extra * (base + 1) ? x / (base + 1) : extra + (x - extra * (base + 1)) / base; }
 };
+
+__device__ __forceinline__ int units(const DecParams& p, int b) {
+  return (int)((min((long)max(p.lens[b], 0), (long)p.max_pages * p.P) + UNIT - 1) / UNIT);
+}
 
 // Not volatile: the products may move behind later ldmatrix loads, which keep their order.
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -295,8 +310,9 @@ struct Loader {
   int page;              // its page, fetched ahead; -1: nothing to load
 };
 
+// 192 registers a thread leave room for a CTA of merge_k on every SM, which waits there for this grid to end.
 template <int NT>
-__global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, DecParams p) {
+__global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, DecParams p) {
   extern __shared__ char smem_raw[];
   char* sm = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -317,8 +333,13 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
   }
-  pdl_trigger();
+  {  // lengths and block table into L2, a hint that needs no order with earlier kernels: the first two of three dependent reads
+    const long at = ((long)blockIdx.x * blockDim.x + threadIdx.x) * 128;
+    if (at < p.B * 4L) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p.lens) + at));
+    if (at < (long)p.B * p.max_pages * 4) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p.bt) + at));
+  }
   pdl_wait();
+  pdl_trigger();  // after the wait: merge_k reads the lengths before this grid ends
   {
     const int per = (p.B + NW * 32 - 1) / (NW * 32), b0 = threadIdx.x * per;
     int sum = 0;
@@ -345,16 +366,10 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     if (threadIdx.x == NW * 32 - 1) prefix[p.B] = before;
     __syncthreads();
   }
-  // as few ranges as the longest one allows, so that nearly all have its length: the last units of a few longer ranges would
-  // run alone (two contexts of 100k: 20 units a warp and 21 for 35 of 1184 cost 3 of 72 us)
-  const int W = prefix[p.B] * p.Hkv, top = (W + gridDim.x * NW - 1) / (gridDim.x * NW), nr = W > 0 ? (W + top - 1) / top : 0;
-  const Ranges rg{W / max(nr, 1), W - W / max(nr, 1) * nr};
-  if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i <= p.B; i += NW * 32) p.plan[i] = prefix[i];
-    if (threadIdx.x == 0) p.plan[p.B + 1] = rg.base, p.plan[p.B + 2] = rg.extra;
-  }
+  const int W = prefix[p.B] * p.Hkv;
+  const Ranges rg(W, gridDim.x * NW);
   const int r = warp * gridDim.x + blockIdx.x;  // neighbouring ranges on different SMs: few units still use every SM
-  if (r >= nr) return;
+  if (r >= rg.n) return;
   const int x0 = rg.lo(r), n_units = rg.lo(r + 1) - x0;
 
   int b, hk, u, U, len;  // unit that is worked on next
@@ -376,7 +391,7 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
   // lane `ch` < chunks loads the box of tokens [ch box, (ch + 1) box) of a unit
   const int chunks = UNIT / p.box;
   const bool loads = lane < chunks;
-  const int pi0 = lane * p.box / p.P, off0 = lane * p.box % p.P;
+  const int pi0 = (unsigned)(lane * p.box) / (unsigned)p.P, off0 = lane * p.box - pi0 * p.P;
   auto fetch_page = [&](Loader& x) {
     x.page = -1;
     if (loads && x.u * UNIT + lane * p.box < x.len) {
@@ -397,7 +412,8 @@ __global__ void __launch_bounds__(NW * 32, 1) decode_k(const __grid_constant__ C
     while (x.b < p.B - 1 && prefix[x.b + 1] == prefix[x.b]);
     if (x.b < p.B) x.U = prefix[x.b + 1] - prefix[x.b], x.len = s_len[x.b];
   };
-  Loader ld{b, hk, u, U, len, n_units, (int)(((long)u * UNIT + lane * p.box) / p.P), (int)(((long)u * UNIT + lane * p.box) % p.P), -1};
+  const unsigned t0 = (unsigned)u * UNIT + lane * p.box;
+  Loader ld{b, hk, u, U, len, n_units, (int)(t0 / (unsigned)p.P), (int)(t0 % (unsigned)p.P), -1};
   fetch_page(ld);
   int nj = 0, row = -1;     // next tile to load (even: K, odd: V of the same unit), its cache row
   bool new_pair = true;     // of `ld`: its q rows come with its K tile
@@ -653,11 +669,25 @@ constexpr int MW = 8, MBATCH = 4;
 __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
   __shared__ float s_o[MW][D];
   __shared__ float2 s_ml[MW];
+  __shared__ int s_sum[2][MW];
   pdl_trigger();
-  pdl_wait();
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = p.plan[b], U = p.plan[b + 1] - first;
-  const Ranges rg{p.plan[p.B + 1], p.plan[p.B + 2]};
+  // units before sequence b, and of all; from the lengths, which decode_k has waited for before it let this grid start
+  int first = 0, all = 0;
+  for (int i = threadIdx.x; i < p.B; i += MW * 32) {
+    const int n = units(p, i);
+    first += i < b ? n : 0;
+    all += n;
+  }
+  first = __reduce_add_sync(0xffffffffu, first), all = __reduce_add_sync(0xffffffffu, all);
+  if (lane == 0) s_sum[0][warp] = first, s_sum[1][warp] = all;
+  __syncthreads();
+  first = all = 0;
+#pragma unroll
+  for (int w = 0; w < MW; ++w) first += s_sum[0][w], all += s_sum[1][w];
+  const int U = units(p, b);
+  const Ranges rg(all * p.Hkv, p.ranges);
+  pdl_wait();
   bf16* out = p.out + ((long)b * p.Hkv + hk) * p.G * D;
   if (U == 0) {
     for (int i = threadIdx.x; i < p.G * D / 8; i += MW * 32) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
@@ -742,97 +772,106 @@ static Cache checked(const at::Tensor& k, const at::Tensor& v, const at::Tensor&
   AX_CHECK((reinterpret_cast<uintptr_t>(k.data_ptr()) & 15) == 0 && (reinterpret_cast<uintptr_t>(v.data_ptr()) & 15) == 0, "fp8 cache: k, v start on a 16-byte boundary");
   return Cache{(uint8_t*)k.data_ptr(), (uint8_t*)v.data_ptr(), (uint8_t*)ks.data_ptr(), (uint8_t*)vs.data_ptr(), (long)k.size(0), (int)k.size(1), (int)k.size(2)};
 }
+// In the given type and contiguous; itself if it is.
+static at::Tensor as(const at::Tensor& t, at::ScalarType ty) { return t.scalar_type() == ty ? t.contiguous() : t.to(ty).contiguous(); }
 static void aligned16(const at::Tensor& t, const char* name) {
   AX_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, name, " starts on a 16-byte boundary");
 }
 
 }  // namespace kv8
 
-std::vector<at::Tensor> qknorm_rope_cache_fp8(at::Tensor qkv, at::Tensor qw, at::Tensor kw, at::Tensor pos, at::Tensor inv_freq, int64_t nq,
-                                              int64_t nkv, double eps, at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor slots,
-                                              bool want_kv) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qknorm_rope_cache_fp8(const at::Tensor& qkv_, const at::Tensor& qw_, const at::Tensor& kw_,
+                                                                     const at::Tensor& pos_, const at::Tensor& inv_freq_, int64_t nq,
+                                                                     int64_t nkv, double eps, const at::Tensor& k, const at::Tensor& v,
+                                                                     const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& slots_,
+                                                                     bool want_kv) {
   using namespace kv8;
   const Cache c = checked(k, v, ks, vs);
   const auto dev = k.device();
+  for (const at::Tensor* t : {&qkv_, &qw_, &kw_, &pos_, &inv_freq_, &slots_}) AX_CHECK(t->device() == dev, "inputs on the cache's device");
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto qkv = qkv_.contiguous(), qw = as(qw_, at::kBFloat16), kw = as(kw_, at::kBFloat16), pos = as(pos_, at::kInt),
+             inv_freq = as(inv_freq_, at::kFloat), slots = as(slots_, at::kLong);
   AX_CHECK(nq >= 0 && nkv >= 1 && nkv == c.Hkv, "nkv must be the cache's head count");
-  AX_CHECK(qkv.device() == dev && qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 2 && qkv.is_contiguous() && qkv.size(1) == (nq + 2 * nkv) * D,
-           "qkv: contiguous bf16 (T, (nq + 2 nkv) 128) on the cache's device");
+  AX_CHECK(qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 2 && qkv.size(1) == (nq + 2 * nkv) * D, "qkv: bf16 (T, (nq + 2 nkv) 128)");
   const int64_t T = qkv.size(0);
   AX_CHECK(T < (1LL << 31), "too many tokens");
-  for (const at::Tensor* w : {&qw, &kw})
-    AX_CHECK(w->device() == dev && w->scalar_type() == at::kBFloat16 && w->numel() == D && w->is_contiguous(), "norm weights: contiguous bf16 (128,) on the cache's device");
-  AX_CHECK(pos.device() == dev && pos.scalar_type() == at::kInt && pos.numel() == T && pos.is_contiguous(), "pos: contiguous int32 (T,)");
-  AX_CHECK(inv_freq.device() == dev && inv_freq.scalar_type() == at::kFloat && inv_freq.numel() == D / 2 && inv_freq.is_contiguous(), "inv_freq: contiguous fp32 (64,)");
-  AX_CHECK(slots.device() == dev && slots.scalar_type() == at::kLong && slots.numel() == T && slots.is_contiguous(), "slots: contiguous int64 (T,)");
+  AX_CHECK(qw.numel() == D && kw.numel() == D && inv_freq.numel() == D / 2, "norm weights (128,), inv_freq (64,)");
+  AX_CHECK(pos.numel() == T && slots.numel() == T, "pos, slots: (T,)");
   aligned16(qkv, "qkv"), aligned16(qw, "q norm weight"), aligned16(kw, "k norm weight");
-  const c10::cuda::CUDAGuard guard(dev);
   const auto opt = qkv.options();
   auto q = at::empty({T, nq, D}, opt);
-  auto ko = at::empty({want_kv ? T : 0, nkv, D}, opt), vo = at::empty({want_kv ? T : 0, nkv, D}, opt);
+  at::Tensor ko, vo;
+  if (want_kv) ko = at::empty({T, nkv, D}, opt), vo = at::empty({T, nkv, D}, opt);
   if (T == 0) return {q, ko, vo};
   const int groups = (int)((nq + 2 * nkv + 3) / 4);
   // warps per token: enough of them to fill the GPU when tokens are few
   const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(groups, (int64_t)num_sms() * 16 / T));
   const long warps = T * (long)parts;
   launch_pdl(append_k, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream(), (const bf16*)qkv.data_ptr(), (const bf16*)qw.data_ptr(),
-             (const bf16*)kw.data_ptr(), (const int*)pos.data_ptr<int>(), (const float*)inv_freq.data_ptr<float>(), (bf16*)q.data_ptr(),
+             (const bf16*)kw.data_ptr(), (const int*)pos.data_ptr(), (const float*)inv_freq.data_ptr(), (bf16*)q.data_ptr(),
              (bf16*)(want_kv ? ko.data_ptr() : nullptr), (bf16*)(want_kv ? vo.data_ptr() : nullptr), (int)T, (int)nq, (int)nkv, (float)eps, c,
-             (const int64_t*)slots.data_ptr<int64_t>(), parts);
+             (const int64_t*)slots.data_ptr(), parts);
   AX_LAUNCH_OK();
   return {q, ko, vo};
 }
 
-void gather_kv_fp8(at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor slots, at::Tensor ko, at::Tensor vo) {
+std::tuple<at::Tensor, at::Tensor> gather_kv_fp8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
+                                                 const at::Tensor& slots_, const c10::optional<at::Tensor>& out_k,
+                                                 const c10::optional<at::Tensor>& out_v) {
   using namespace kv8;
   const Cache c = checked(k, v, ks, vs);
   const auto dev = k.device();
-  AX_CHECK(slots.device() == dev && slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous(), "slots: contiguous int64 (T,)");
+  AX_CHECK(slots_.device() == dev && slots_.dim() == 1, "slots: (T,) on the cache's device");
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto slots = as(slots_, at::kLong);
   const long T = slots.numel();
+  const auto opt = k.options().dtype(at::kBFloat16);
+  auto ko = out_k.has_value() ? *out_k : at::empty({T, c.Hkv, D}, opt), vo = out_v.has_value() ? *out_v : at::empty({T, c.Hkv, D}, opt);
   for (const at::Tensor* o : {&ko, &vo}) {
     AX_CHECK(o->device() == dev && o->scalar_type() == at::kBFloat16 && o->dim() == 3 && o->size(0) == T && o->size(1) == c.Hkv && o->size(2) == D && o->is_contiguous(),
              "outputs: contiguous bf16 (T, Hkv, 128) on the cache's device");
     aligned16(*o, "output");
   }
-  if (T == 0 || c.Hkv == 0) return;
-  const c10::cuda::CUDAGuard guard(dev);
+  if (T == 0 || c.Hkv == 0) return {ko, vo};
   const long n = T * c.Hkv * 16;
-  load_k<<<(unsigned)std::min<long>((n + 255) / 256, (long)num_sms() * 32), 256, 0, stream()>>>(c, slots.data_ptr<int64_t>(), (bf16*)ko.data_ptr(),
-                                                                                               (bf16*)vo.data_ptr(), T);
+  launch_pdl(load_k, dim3((unsigned)std::min<long>((n + 255) / 256, (long)num_sms() * 32)), dim3(256), 0, stream(), c,
+             (const int64_t*)slots.data_ptr(), (bf16*)ko.data_ptr(), (bf16*)vo.data_ptr(), T);
   AX_LAUNCH_OK();
+  return {ko, vo};
 }
 
-at::Tensor paged_decode_attn_fp8(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor ks, at::Tensor vs, at::Tensor block_table, at::Tensor seq_lens,
-                                 double scale) {
+at::Tensor paged_decode_attn_fp8(const at::Tensor& q_, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
+                                 const at::Tensor& block_table_, const at::Tensor& seq_lens_, double scale) {
   using namespace kv8;
   const Cache c = checked(k, v, ks, vs);
   const auto dev = k.device();
-  AX_CHECK(q.device() == dev && q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.size(2) == D && q.is_contiguous(), "q: contiguous bf16 (B, Hq, 128) on the cache's device");
+  for (const at::Tensor* t : {&q_, &block_table_, &seq_lens_}) AX_CHECK(t->device() == dev, "inputs on the cache's device");
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto q = q_.contiguous(), block_table = block_table_.contiguous(), seq_lens = seq_lens_.contiguous();
+  AX_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.size(2) == D, "q: bf16 (B, Hq, 128)");
   const int64_t B = q.size(0), Hq = q.size(1);
   AX_CHECK(c.Hkv >= 1 && Hq >= 1 && Hq % c.Hkv == 0 && Hq / c.Hkv <= MAXG, "GQA group must be <= 16");
-  AX_CHECK(block_table.device() == dev && block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == B && block_table.is_contiguous(),
-           "block_table: contiguous int32 (B, pages)");
-  AX_CHECK(seq_lens.device() == dev && seq_lens.scalar_type() == at::kInt && seq_lens.numel() == B && seq_lens.is_contiguous(), "seq_lens: contiguous int32 (B,)");
+  AX_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == B, "block_table: int32 (B, pages)");
+  AX_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.numel() == B, "seq_lens: int32 (B,)");
   AX_CHECK(c.P % 16 == 0 && c.P > 0, "page size must be a multiple of 16");
-  aligned16(q, "q");
-  AX_CHECK((reinterpret_cast<uintptr_t>(ks.data_ptr()) & 15) == 0 && (reinterpret_cast<uintptr_t>(vs.data_ptr()) & 15) == 0, "fp8 cache: scales start on a 16-byte boundary");
+  aligned16(q, "q"), aligned16(ks, "fp8 cache: scale tensor"), aligned16(vs, "fp8 cache: scale tensor");
   AX_CHECK(B <= MAXB, "decode batch must be <= ", MAXB);
   const long rows = c.pages * c.Hkv * c.P;
   AX_CHECK(rows < (1L << 31), "fp8 cache: pages * Hkv * page size must be below 2^31");
   AX_CHECK(B * (block_table.size(1) * c.P / UNIT + 1) * c.Hkv < (1L << 31), "block_table: too many tokens");
-  const c10::cuda::CUDAGuard guard(dev);
   auto out = at::empty_like(q);
   if (B == 0) return out;
   if (rows == 0 || block_table.size(1) == 0) return out.zero_();
-  const int G = (int)(Hq / c.Hkv), grid = num_sms();
-  const long ranges = (long)grid * NW;
-  // freed after the launches, so the memory is handed on in stream order (and belongs to the graph when captured)
-  auto part_o = at::empty({ranges * 2 * G * D}, q.options().dtype(at::kFloat)), part_ml = at::empty({ranges * 2 * G * 2}, part_o.options());
-  auto plan = at::empty({B + 3}, q.options().dtype(at::kInt));
+  const int G = (int)(Hq / c.Hkv), grid = num_sms(), ranges = grid * NW;
+  // partials: freed after the launches, so the memory is handed on in stream order (and is the graph's when captured)
+  const long floats = (long)ranges * 2 * G * D;
+  const c10::DataPtr part = c10::cuda::CUDACachingAllocator::get()->allocate((floats + (long)ranges * 2 * G * 2) * sizeof(float));
   int box = 16;
   while (box < 64 && c.P % (2 * box) == 0) box *= 2;
   const CUtensorMap tk = codes_map(c.k, rows, box), tv = codes_map(c.v, rows, box);
-  const DecParams p{(const bf16*)q.data_ptr(), block_table.data_ptr<int>(), seq_lens.data_ptr<int>(), c.ks, c.vs, (bf16*)out.data_ptr(),
-                    part_o.data_ptr<float>(), (float2*)part_ml.data_ptr<float>(), plan.data_ptr<int>(), c.pages, (int)B, G, c.Hkv, c.P,
+  const DecParams p{(const bf16*)q.data_ptr(), (const int*)block_table.data_ptr(), (const int*)seq_lens.data_ptr(), c.ks, c.vs, (bf16*)out.data_ptr(),
+                    (float*)part.get(), (float2*)((float*)part.get() + floats), ranges, c.pages, (int)B, G, c.Hkv, c.P,
                     (int)block_table.size(1), box, (float)(scale * 1.4426950408889634)};
   auto kern = G <= 8 ? decode_k<1> : decode_k<2>;
   smem_attr((const void*)kern, DEC_SMEM);

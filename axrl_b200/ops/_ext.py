@@ -87,6 +87,7 @@ class _Counting:
                 _COUNT["launches"] += _KERNELS_PER_CALL.get(name, 1)
             return fn(*a, **k)
 
+        self.__dict__[name] = wrapped  # looked up without __getattr__ from now on
         return wrapped
 
     @property

@@ -107,17 +107,13 @@ def qk_norm_rope_cache_fp8(qkv: torch.Tensor, qw: torch.Tensor, kw: torch.Tensor
         k = _rope64(_rms_ref(k, kw, eps), pos, inv_freq)
         k, v = _append_ref(cache, k, v, slots.long())
         return (q, k.to(qkv.dtype), v.to(qkv.dtype)) if want_kv else (q, None, None)
-    bf = torch.bfloat16
-    q, k, v = _ext.ext().qknorm_rope_cache_fp8(qkv.contiguous(), qw.to(bf).contiguous(), kw.to(bf).contiguous(), pos.to(torch.int32).contiguous(),
-                                               inv_freq.float().contiguous(), nq, nkv, eps, *cache, slots.long().contiguous(), want_kv)
-    return (q, k, v) if want_kv else (q, None, None)
+    return _ext.ext().qknorm_rope_cache_fp8(qkv, qw, kw, pos, inv_freq, nq, nkv, eps, *cache, slots, want_kv)
 
 
 def gather_kv_fp8(cache: Fp8KV, slots: torch.Tensor, out_k: torch.Tensor | None = None, out_v: torch.Tensor | None = None
                   ) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows of the cache at ``slots`` (T,) as bf16 ``k, v (T, Hkv, 128)`` (exact; zeros for a slot outside the cache), for a
     prefill that continues a cached prefix.  ``out_k`` / ``out_v``: contiguous tensors to write to instead of new ones."""
-    shape = (slots.numel(), cache.k.shape[1], cache.k.shape[3])
     if not cache.k.is_cuda:
         live = _live(cache, slots)
         at = torch.where(live, slots, torch.zeros_like(slots)).long()
@@ -127,10 +123,7 @@ def gather_kv_fp8(cache: Fp8KV, slots: torch.Tensor, out_k: torch.Tensor | None 
             x = torch.where(live[:, None, None], x, torch.zeros_like(x))
             res.append(x if out is None else out.copy_(x))
         return res[0], res[1]
-    k = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device) if out_k is None else out_k
-    v = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device) if out_v is None else out_v
-    _ext.ext().gather_kv_fp8(*cache, slots.long().contiguous(), k, v)
-    return k, v
+    return _ext.ext().gather_kv_fp8(*cache, slots, out_k, out_v)
 
 
 def decode_attention_fp8_ref(q: torch.Tensor, cache: Fp8KV, block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float) -> torch.Tensor:
@@ -160,4 +153,4 @@ def paged_decode_attention_fp8(q: torch.Tensor, cache: Fp8KV, block_table: torch
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if not q.is_cuda:
         return decode_attention_fp8_ref(q, cache, block_table, seq_lens, scale)
-    return _ext.ext().paged_decode_attn_fp8(q.contiguous(), *cache, block_table, seq_lens, scale)
+    return _ext.ext().paged_decode_attn_fp8(q, *cache, block_table, seq_lens, scale)
