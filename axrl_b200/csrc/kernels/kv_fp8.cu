@@ -56,78 +56,105 @@ struct Cache {
 };
 
 // ----------------------------------------------------------------------------- append
-// One quarter-warp per (token, head): lane l of 8 holds elements 8l .. 8l + 7 of both halves, so a
-// rotation pair stays in one thread and every access is 16 bytes (codes: 8).  The four quarters of a
-// warp take four heads at a time; the angles of the token are computed once per warp.
-//   n = x rsqrt(mean x^2 + eps) w;  rotated by pos * inv_freq (angle reduced in 64 bits: at position
-//   10^5 a 32-bit angle is off by 4e-3);  code = rne(x / scale), one rounding from the fp32 value.
-__global__ void __launch_bounds__(256) append_k(const bf16* __restrict__ qkv, const bf16* __restrict__ qw, const bf16* __restrict__ kw,
-                                                const int* __restrict__ pos, const float* __restrict__ inv_freq, bf16* __restrict__ q,
-                                                bf16* __restrict__ ko, bf16* __restrict__ vo, int T, int nq, int nkv, float eps, Cache c,
-                                                const int64_t* __restrict__ slots, int parts) {
+//   n = x rsqrt(mean x^2 + eps) w;  rotated by pos * inv_freq;  code = rne(x / scale), one rounding from the fp32 value.
+// Moves (nq + 2 nkv) 256 bytes a token in and nq 256 + nkv 258 (+ nkv 512) out; bound by that for many tokens.  A CTA of
+// eight warps takes 8 / parts tokens, `parts` warps each.  Its threads first put the products of each token's 64 angles
+// (reduced in 64 bits: at position 10^5 a 32-bit angle is off by 4e-3) with both norm weights into shared memory, once per
+// token: a' = r (a wa cos - b wb sin), b' = r (b wb cos + a wa sin).  A warp works on four heads at a time, a quarter-warp
+// each: lane l of 8 holds elements 8l .. 8l + 7 of both halves, so a rotation pair stays in one thread and every access is 16
+// bytes (codes: 8); the next four heads are loaded before the current ones are computed.  16384 tokens of 32 q and 8 kv
+// heads: one warp walking a token with its own angles 100 us, products in registers 113 us (14 warps an SM), this form TODO.
+constexpr int AW = 8;  // warps
+
+// Largest magnitude, a NaN if there is one (the sign of the result means nothing).
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__global__ void __launch_bounds__(AW * 32, 4) append_k(const bf16* __restrict__ qkv, const bf16* __restrict__ qw, const bf16* __restrict__ kw,
+                                                       const int* __restrict__ pos, const float* __restrict__ inv_freq, bf16* __restrict__ q,
+                                                       bf16* __restrict__ ko, bf16* __restrict__ vo, int T, int nq, int nkv, float eps, Cache c,
+                                                       const int64_t* __restrict__ slots, int parts) {
+  // [token][q, k][i][l]: wa cos, wb sin, wb cos, wa sin of pair 8 l + i; eight lanes read 128 consecutive bytes
+  __shared__ float4 s_w[AW / 2][2][8][8];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l8 = lane & 7;
-  const long warp = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  if (warp >= (long)T * parts) return;
-  const int t = (int)(warp / parts), part = (int)(warp % parts);
-  const int nh = nq + 2 * nkv;
-  const int groups = (nh + 3) >> 2;  // of four heads
-  const int g0 = (int)((long)groups * part / parts), g1 = (int)((long)groups * (part + 1) / parts);
-  float cs[8], sn[8];
-  {
-    const double turns_per_pos = 0.15915494309189535;  // 1 / (2 pi)
-    const double p = (double)pos[t] * turns_per_pos;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      double a = p * (double)inv_freq[8 * l8 + i];
-      a -= rint(a);
-      sincospif((float)(2.0 * a), &sn[i], &cs[i]);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7, tokens = AW / parts;
+  const int t0 = blockIdx.x * tokens;
+  const int tt = warp / parts, part = warp % parts, t = t0 + tt;
+  const int gq = (nq + 3) >> 2, gk = (nkv + 3) >> 2, groups = gq + 2 * gk;  // of four heads: q, then k, then v
+  const int g0 = groups * part / parts, g1 = groups * (part + 1) / parts;
+  const bool any = t < T && g0 < g1;
+  const bf16* src = qkv + (long)t * (nq + 2 * nkv) * D + 8 * l8;
+  uint4 na = make_uint4(0, 0, 0, 0), nb = na;
+  auto fetch = [&](int g) {
+    const int skip = g < gq ? 0 : g < gq + gk ? gq : gq + gk, h = 4 * (g - skip) + (lane >> 3);
+    if (h < (g < gq ? nq : nkv)) {
+      const bf16* at = src + (h + (g < gq ? 0 : g < gq + gk ? nq : nq + nkv)) * D;
+      na = *reinterpret_cast<const uint4*>(at), nb = *reinterpret_cast<const uint4*>(at + 64);
     }
-  }
-  const long slot = slots[t];
-  const bool live = slot >= 0 && slot < c.pages * c.P;
-  const long page = live ? slot / c.P : 0, off = live ? slot % c.P : 0;
-  for (int g = g0; g < g1; ++g) {
-    const int h = g * 4 + (lane >> 3);
-    const bool in = h < nh;
-    const int hh = in ? h : nh - 1;
-    const bf16* src = qkv + ((long)t * nh + hh) * D + 8 * l8;
-    float a[8], b[8];
-    load8(src, a);
-    load8(src + 64, b);
-    const bool isv = hh >= nq + nkv, isq = hh < nq;
-    float ss = 0.f;
+  };
+  if (any) fetch(g0);
+  const long slot = any ? slots[t] : -1;
+  if ((int)threadIdx.x < tokens * (D / 2)) {
+    const int ti = threadIdx.x / (D / 2), f = threadIdx.x % (D / 2);
+    if (t0 + ti < T) {
+      double a = (double)pos[t0 + ti] * 0.15915494309189535 * (double)inv_freq[f];  // in turns: 1 / (2 pi)
+      a -= rint(a);
+      float sn, cs;
+      sincospif((float)(2.0 * a), &sn, &cs);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!isv) {
-      const float r = rsqrtf(ss / D + eps);
-      const bf16* w = isq ? qw : kw;
-      float wa[8], wb[8];
-      load8(w + 8 * l8, wa);
-      load8(w + 64 + 8 * l8, wb);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = a[i] * r * wa[i], y = b[i] * r * wb[i];
-        a[i] = x * cs[i] - y * sn[i];
-        b[i] = y * cs[i] + x * sn[i];
+      for (int k = 0; k < 2; ++k) {
+        const bf16* w = k ? kw : qw;
+        const float wa = __bfloat162float(w[f]), wb = __bfloat162float(w[f + 64]);
+        s_w[ti][k][f & 7][f >> 3] = make_float4(wa * cs, wb * sn, wb * cs, wa * sn);
       }
     }
-    uint32_t m = 0;
+  }
+  const bool live = slot >= 0 && slot < c.pages * c.P;
+  const long row0 = live ? slot / c.P * c.Hkv * c.P + slot % c.P : 0;  // cache row of head 0
+  __syncthreads();
+  if (!any) return;
+  for (int g = g0; g < g1; ++g) {
+    const bool isq = g < gq, isv = g >= gq + gk;
+    const int h = 4 * (g - (isq ? 0 : isv ? gq + gk : gq)) + (lane >> 3);
+    const bool in = h < (isq ? nq : nkv);
+    float a[8], b[8];
+    load8(reinterpret_cast<const bf16*>(&na), a);
+    load8(reinterpret_cast<const bf16*>(&nb), b);
+    if (g + 1 < g1) fetch(g + 1);
+    if (!isv) {
+      float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, max(__float_as_uint(fabsf(a[i])), __float_as_uint(fabsf(b[i]))));
+      for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (!in) continue;
+      for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(ss / D + eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 w = s_w[tt][isq ? 0 : 1][i][l8];
+        const float x = a[i] * r, y = b[i] * r;
+        a[i] = x * w.x - y * w.y;
+        b[i] = y * w.z + x * w.w;
+      }
+    }
     if (isq) {
-      bf16* dst = q + ((long)t * nq + hh) * D + 8 * l8;
-      store8(dst, a);
-      store8(dst + 64, b);
+      if (in) {
+        bf16* dst = q + ((long)t * nq + h) * D + 8 * l8;
+        store8(dst, a);
+        store8(dst + 64, b);
+      }
       continue;
     }
-    const int hv = hh - nq - (isv ? nkv : 0);
+    float top = max_abs(a[0], b[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = max_abs(top, max_abs(a[i], b[i]));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const uint32_t m = __float_as_uint(top) & 0x7fffffffu;
+    if (!in) continue;
     const uint32_t e = scale_byte(m);
     const float inv = inv_scale(e);
     uint32_t ca[2] = {0, 0}, cb[2] = {0, 0};
@@ -139,7 +166,7 @@ __global__ void __launch_bounds__(256) append_k(const bf16* __restrict__ qkv, co
       }
     }
     if (live) {
-      const long row = (page * c.Hkv + hv) * c.P + off;
+      const long row = row0 + (long)h * c.P;
       uint8_t* dst = (isv ? c.v : c.k) + row * D + 8 * l8;
       *reinterpret_cast<uint2*>(dst) = make_uint2(ca[0], ca[1]);
       *reinterpret_cast<uint2*>(dst + 64) = make_uint2(cb[0], cb[1]);
@@ -152,7 +179,7 @@ __global__ void __launch_bounds__(256) append_k(const bf16* __restrict__ qkv, co
         const float2 x = from_e4m3x2(ca[i >> 1] >> (16 * (i & 1))), y = from_e4m3x2(cb[i >> 1] >> (16 * (i & 1)));
         a[2 * i] = x.x * s, a[2 * i + 1] = x.y * s, b[2 * i] = y.x * s, b[2 * i + 1] = y.y * s;
       }
-      bf16* dst = (isv ? vo : ko) + ((long)t * nkv + hv) * D + 8 * l8;
+      bf16* dst = (isv ? vo : ko) + ((long)t * nkv + h) * D + 8 * l8;
       store8(dst, a);
       store8(dst + 64, b);
     }
@@ -160,36 +187,47 @@ __global__ void __launch_bounds__(256) append_k(const bf16* __restrict__ qkv, co
 }
 
 // ----------------------------------------------------------------------------- load
-// Rows of the cache as bf16: one thread per 16 codes of K or V; exact.
-__global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict__ slots, bf16* __restrict__ ko, bf16* __restrict__ vo, long T) {
+// Rows of the cache as bf16 (exact): 129 bytes in and 256 out for each of the 2 Hkv rows of a slot, bound by that.  A warp
+// takes 16 rows (the rows of one slot with eight heads): lane i looks up row i, then two rows at a time are converted, 16
+// lanes of 8 codes each, so that a store fills 512 bytes; all 16 rows are read before the first is written.  One thread per
+// 16 codes, each looking up its own slot, took 395 us for 131072 slots (floor 123), this form TODO.
+constexpr int LR = 16;
+
+__global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict__ slots, bf16* __restrict__ ko, bf16* __restrict__ vo, long rows) {
   pdl_trigger();
   pdl_wait();
-  const long n = T * c.Hkv * 16;  // 8 chunks of 16 codes for K, then for V
-  for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) {
-    const int ch = (int)(i & 7), isv = (int)(i >> 3) & 1;
-    const long th = i >> 4;
-    const int h = (int)(th % c.Hkv);
-    const long t = th / c.Hkv;
+  const int lane = threadIdx.x & 31;
+  const long base = (((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5) * LR;  // rows: (slot, K or V, head)
+  if (base >= rows) return;
+  const long r = base + (lane & 15);
+  const uint8_t* src = nullptr;  // nothing to read: zeros
+  bf16* dst = nullptr;
+  float scale = 0.f;
+  if (r < rows) {
+    const long t = r / (2 * c.Hkv);
+    const int j = (int)(r - t * 2 * c.Hkv), isv = j >= c.Hkv, h = j - isv * c.Hkv;
+    dst = (isv ? vo : ko) + (t * c.Hkv + h) * D;
     const long slot = slots[t];
-    uint4 w = make_uint4(0, 0, 0, 0);
-    float s = 0.f;
     if (slot >= 0 && slot < c.pages * c.P) {
-      const long row = ((slot / c.P) * c.Hkv + h) * c.P + slot % c.P;
-      w = *reinterpret_cast<const uint4*>((isv ? c.v : c.k) + row * D + ch * 16);
-      s = scale_value((isv ? c.vs : c.ks)[row]);
+      const long page = slot / c.P, row = (page * c.Hkv + h) * c.P + (slot - page * c.P);
+      src = (isv ? c.v : c.k) + row * D;
+      scale = scale_value((isv ? c.vs : c.ks)[row]);
     }
-    bf16* dst = (isv ? vo : ko) + th * D + ch * 16;
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+  }
+  uint2 w[LR / 2];
+  const int l16 = lane & 15;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float f[8];
+  for (int i = 0; i < LR / 2; ++i) {
+    const uint8_t* p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, (unsigned long long)src, 2 * i + (lane >> 4)));
+    w[i] = p != nullptr ? *reinterpret_cast<const uint2*>(p + 8 * l16) : make_uint2(0, 0);
+  }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x = from_e4m3x2(ws[2 * half + (j >> 1)] >> (16 * (j & 1)));
-        f[2 * j] = x.x * s, f[2 * j + 1] = x.y * s;
-      }
-      store8(dst + 8 * half, f);
-    }
+  for (int i = 0; i < LR / 2; ++i) {
+    bf16* d = reinterpret_cast<bf16*>(__shfl_sync(0xffffffffu, (unsigned long long)dst, 2 * i + (lane >> 4)));
+    const float s = __shfl_sync(0xffffffffu, scale, 2 * i + (lane >> 4));
+    const float2 x0 = from_e4m3x2(w[i].x), x1 = from_e4m3x2(w[i].x >> 16), x2 = from_e4m3x2(w[i].y), x3 = from_e4m3x2(w[i].y >> 16);
+    const float f[8] = {x0.x * s, x0.y * s, x1.x * s, x1.y * s, x2.x * s, x2.y * s, x3.x * s, x3.y * s};
+    if (d != nullptr) store8(d + 8 * l16, f);
   }
 }
 
@@ -804,11 +842,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qknorm_rope_cache_fp8(const at::T
   at::Tensor ko, vo;
   if (want_kv) ko = at::empty({T, nkv, D}, opt), vo = at::empty({T, nkv, D}, opt);
   if (T == 0) return {q, ko, vo};
-  const int groups = (int)((nq + 2 * nkv + 3) / 4);
-  // warps per token: enough of them to fill the GPU when tokens are few
-  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(groups, (int64_t)num_sms() * 16 / T));
-  const long warps = T * (long)parts;
-  launch_pdl(append_k, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream(), (const bf16*)qkv.data_ptr(), (const bf16*)qw.data_ptr(),
+  // Warps per token: eight until the SMs have some sixteen CTAs each (a single token: 2.9 us either way), then fewer, which
+  // share the products of weights and angles among more heads (16384 tokens: TODO).
+  const int64_t many = (int64_t)num_sms() * 4;
+  const int parts = T <= many ? 8 : T <= 2 * many ? 4 : 2;
+  launch_pdl(append_k, dim3((unsigned)((T + AW / parts - 1) / (AW / parts))), dim3(AW * 32), 0, stream(), (const bf16*)qkv.data_ptr(), (const bf16*)qw.data_ptr(),
              (const bf16*)kw.data_ptr(), (const int*)pos.data_ptr(), (const float*)inv_freq.data_ptr(), (bf16*)q.data_ptr(),
              (bf16*)(want_kv ? ko.data_ptr() : nullptr), (bf16*)(want_kv ? vo.data_ptr() : nullptr), (int)T, (int)nq, (int)nkv, (float)eps, c,
              (const int64_t*)slots.data_ptr(), parts);
@@ -834,9 +872,9 @@ std::tuple<at::Tensor, at::Tensor> gather_kv_fp8(const at::Tensor& k, const at::
     aligned16(*o, "output");
   }
   if (T == 0 || c.Hkv == 0) return {ko, vo};
-  const long n = T * c.Hkv * 16;
-  launch_pdl(load_k, dim3((unsigned)std::min<long>((n + 255) / 256, (long)num_sms() * 32)), dim3(256), 0, stream(), c,
-             (const int64_t*)slots.data_ptr(), (bf16*)ko.data_ptr(), (bf16*)vo.data_ptr(), T);
+  const long rows = T * 2 * c.Hkv, ctas = (rows + 8 * LR - 1) / (8 * LR);
+  AX_CHECK(ctas < (1L << 31), "too many slots");
+  launch_pdl(load_k, dim3((unsigned)ctas), dim3(256), 0, stream(), c, (const int64_t*)slots.data_ptr(), (bf16*)ko.data_ptr(), (bf16*)vo.data_ptr(), rows);
   AX_LAUNCH_OK();
   return {ko, vo};
 }
