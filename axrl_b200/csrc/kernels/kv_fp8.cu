@@ -235,10 +235,10 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // o = sum_t softmax_t(scale q.k_t) v_t with k_t = kc_t 2^{a_t}, v_t = vc_t 2^{e_t} (codes, exponents).
 //
 // Work: unit = 64 tokens of one (sequence, kv head).  The units of all (sequence, kv head) pairs in a row form
-// one list, cut into equal contiguous ranges, one per warp of the grid (one CTA per SM): every warp streams
-// the same number of bytes whatever the lengths are.  A pair that lies inside one range is finished by its warp; the
-// others leave fp32 partials (at most two per warp), which merge_k combines.  A warp works alone: its own ring
-// of 8 KB slots (K and V tiles in turn) filled by its own TMA loads (128-byte swizzle), no barrier with other warps.
+// one list, cut into contiguous ranges of equal cost, one per warp of the grid (one CTA per SM): every warp is busy equally
+// long whatever the lengths are.  A pair that lies inside one range is finished by its warp; the others leave fp32
+// partials (at most two per warp), which merge_k combines.  A warp works alone: its own ring of 8 KB slots (K and V tiles
+// in turn) filled by its own TMA loads (128-byte swizzle), no barrier with other warps.
 //
 // Both products are m16n8k16 with f16 operands and fp32 sums; f16 holds every e4m3 code exactly:
 //   S^T (tokens x heads) = Kc Q^T,   O^T (dims x heads) += Vc^T P^T
@@ -285,20 +285,21 @@ __device__ __forceinline__ bool wait_tile(uint64_t* bar, uint32_t phase) {
     }
   return true;
 }
-// W units in n ranges of `base` units, the first `extra` of them one longer.  As few ranges as the longest one allows, so
-// that nearly all have its length: the last units of a few longer ranges would run alone (two contexts of 100k: 20 units a
-// warp and 21 for 35 of 1184 cost 2 of 72 us).
+// Costs are counted in cells: two for a unit and one for each pair (its q, its output; measured 2.4 to 2.8 us a unit and 1.0 us a
+// pair, and 256 short sequences take 37.3 us with ranges of equal units, 35.3 us with equal cells).  Cell 0 of a pair is its own,
+// unit u starts at cell 1 + 2 u, and a range does the units that start in it.  All ranges have the same even length, so as few
+// as possible: with lengths that differ by a unit the longer ones end alone (two contexts of 100k, 20 and 21 units: 71.2 us,
+// all 21: 69.3 us).  Two cells or more: a range inside a pair has a unit.
 struct Ranges {
-  int n, base, extra;
-  __device__ Ranges(int W, int most) {
-    const int top = max((W + most - 1) / most, 1);
-    n = (W + top - 1) / top;
-    base = W / max(n, 1);
-    extra = W - base * n;
+  int len, n;
+  __device__ Ranges(int cells, int most) : len(((cells + most - 1) / most + 1) & ~1) {
+    len = max(len, 2);
+    n = (cells + len - 1) / len;
   }
-  __device__ int lo(int r) const { return r * base + min(r, extra); }
-  __device__ int of(int x) const { return x < extra * (base + 1) ? x / (base + 1) : extra + (x - extra * (base + 1)) / base; }
+  __device__ int lo(int r) const { return r * len; }
+  __device__ int of(int x) const { return x / len; }
 };
+__device__ __forceinline__ int cells(int units) { return units > 0 ? 2 * units + 1 : 0; }
 
 __device__ __forceinline__ int units(const DecParams& p, int b) {
   return (int)((min((long)max(p.lens[b], 0), (long)p.max_pages * p.P) + UNIT - 1) / UNIT);
@@ -343,7 +344,7 @@ __device__ __forceinline__ void bulk_bytes(void* dst, const void* src, int bytes
 // Position of a warp's loads in its range.
 struct Loader {
   int b, hk, u, U, len;  // unit that is loaded next
-  int left;              // units of the range still to load
+  int left;              // cells of the range from its start on; none left: the range is done
   int pi, off;           // this lane's chunk of that unit: index into the block table, token within the page
   int page;              // its page, fetched ahead; -1: nothing to load
 };
@@ -359,7 +360,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + NW * SLOTS * (TILE + UNIT)) + warp * SLOTS;
   uchar4* meta = reinterpret_cast<uchar4*>(sm + NW * SLOTS * (TILE + UNIT + 8)) + warp * SLOTS;  // which chunks of a slot were loaded
   char* sq = sm + NW * SLOTS * (TILE + UNIT + 12) + warp * Q_BYTES;  // q rows of the pair that is loaded next
-  int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12) + NW * Q_BYTES);  // units of the sequences before
+  int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12) + NW * Q_BYTES);  // cells of a kv head of the sequences before
   int* s_len = prefix + MAXB + 1;
   __shared__ int s_warp[NW];
 
@@ -384,7 +385,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
     for (int i = b0; i < min(b0 + per, p.B); ++i) {
       const int n = (int)min((long)max(p.lens[i], 0), (long)p.max_pages * p.P);
       s_len[i] = n;
-      sum += (n + UNIT - 1) / UNIT;
+      sum += cells((n + UNIT - 1) / UNIT);
     }
     int x = sum;
 #pragma unroll
@@ -399,18 +400,17 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
     for (int w = 0; w < NW; ++w) before += w < warp ? s_warp[w] : 0;
     for (int i = b0; i < min(b0 + per, p.B); ++i) {
       prefix[i] = before;
-      before += (s_len[i] + UNIT - 1) / UNIT;
+      before += cells((s_len[i] + UNIT - 1) / UNIT);
     }
     if (threadIdx.x == NW * 32 - 1) prefix[p.B] = before;
     __syncthreads();
   }
-  const int W = prefix[p.B] * p.Hkv;
-  const Ranges rg(W, gridDim.x * NW);
+  const Ranges rg(prefix[p.B] * p.Hkv, gridDim.x * NW);
   const int r = warp * gridDim.x + blockIdx.x;  // neighbouring ranges on different SMs: few units still use every SM
   if (r >= rg.n) return;
-  const int x0 = rg.lo(r), n_units = rg.lo(r + 1) - x0;
+  const int x0 = rg.lo(r);
 
-  int b, hk, u, U, len;  // unit that is worked on next
+  int b, hk, u, U, len, left;  // unit that is worked on next, cells of the range from its start on
   {
     const int pos = x0 / p.Hkv;  // sequence b: prefix[b] <= pos < prefix[b + 1]
     int lo = 0, n = p.B;  // b in [lo, lo + n)
@@ -421,11 +421,27 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
       lo += k * step;
     }
     b = lo;
-    U = prefix[b + 1] - prefix[b];
-    const int rem = x0 - prefix[b] * p.Hkv;
-    hk = rem / U, u = rem % U;
+    const int pc = prefix[b + 1] - prefix[b], rem = x0 - prefix[b] * p.Hkv;
+    U = pc / 2;
+    hk = rem / pc;
+    const int off = rem - hk * pc;
+    u = off / 2;
+    left = min(rg.lo(r + 1), prefix[p.B] * p.Hkv) - x0 - (1 + 2 * u - off);
     len = s_len[b];
   }
+  auto next_pair = [&](int& b, int& hk, int& u, int& U, int& len) {
+    u = 0;
+    if (++hk < p.Hkv) return;
+    hk = 0;
+    do ++b;
+    while (b < p.B - 1 && prefix[b + 1] == prefix[b]);
+    if (b < p.B) U = (prefix[b + 1] - prefix[b]) / 2, len = s_len[b];
+  };
+  if (u == U) {  // the range starts in the second half of the last unit of a pair
+    next_pair(b, hk, u, U, len);
+    left -= 1;  // its own cell; the start of a unit U had been counted already
+  }
+  if (left <= 0) return;
   // lane `ch` < chunks loads the box of tokens [ch box, (ch + 1) box) of a unit
   const int chunks = UNIT / p.box;
   const bool loads = lane < chunks;
@@ -438,34 +454,32 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
     }
   };
   auto next_unit = [&](Loader& x) {
+    x.left -= 2;
     if (++x.u < x.U) {
       x.off += UNIT;
       while (x.off >= p.P) x.off -= p.P, ++x.pi;
       return;
     }
-    x.u = 0, x.pi = pi0, x.off = off0;
-    if (++x.hk < p.Hkv) return;
-    x.hk = 0;
-    do ++x.b;
-    while (x.b < p.B - 1 && prefix[x.b + 1] == prefix[x.b]);
-    if (x.b < p.B) x.U = prefix[x.b + 1] - prefix[x.b], x.len = s_len[x.b];
+    x.left -= 1;
+    x.pi = pi0, x.off = off0;
+    next_pair(x.b, x.hk, x.u, x.U, x.len);
   };
   const unsigned t0 = (unsigned)u * UNIT + lane * p.box;
-  Loader ld{b, hk, u, U, len, n_units, (int)(t0 / (unsigned)p.P), (int)(t0 % (unsigned)p.P), -1};
+  Loader ld{b, hk, u, U, len, left, (int)(t0 / (unsigned)p.P), (int)(t0 % (unsigned)p.P), -1};
   fetch_page(ld);
   int nj = 0, row = -1;     // next tile to load (even: K, odd: V of the same unit), its cache row
   bool new_pair = true;     // of `ld`: its q rows come with its K tile
   auto load_next = [&] {
     if ((nj & 1) == 0) {
-      if (ld.left == 0) return;
+      if (ld.left <= 0) return;
       if (new_pair && lane == 0) {
         const int bytes = p.G * D * 2;
         tc::mbar_tx(&full[nj % SLOTS], bytes);  // counted before the arrival below completes the phase
         bulk_bytes(sq, p.q + ((long)ld.b * p.Hkv + ld.hk) * p.G * D, bytes, &full[nj % SLOTS]);
       }
       row = ld.page >= 0 ? (int)(((long)ld.page * p.Hkv + ld.hk) * p.P) + ld.off : -1;
-      if (--ld.left > 0) {
-        next_unit(ld);
+      next_unit(ld);
+      if (ld.left > 0) {
         new_pair = ld.u == 0;
         fetch_page(ld);
       }
@@ -498,7 +512,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   uint32_t qf[NT][16];
   bool fresh = true, begun_before = u > 0;  // the pair at the start of the range may have begun in an earlier one
   int j = 0;
-  for (int i = 0; i < n_units; ++i) {
+  while (left > 0) {
     const int sk = j % SLOTS, sv = (j + 1) % SLOTS;
     // --- scores of 64 tokens
     if (!__all_sync(0xffffffffu, wait_tile(&full[sk], (j / SLOTS) & 1))) break;
@@ -658,7 +672,8 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
     j += 2;
     // --- end of the pair, or of the range
     const bool ends = u == U - 1;
-    if (ends || i == n_units - 1) {
+    left -= ends ? 3 : 2;
+    if (ends || left <= 0) {
       const bool whole = ends && !begun_before;
       const int slot = (r * 2 + (begun_before ? 0 : 1)) * p.G;
 #pragma unroll
@@ -684,15 +699,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
       fresh = true;
       begun_before = false;
     }
-    if (++u == U) {
-      u = 0;
-      if (++hk == p.Hkv) {
-        hk = 0;
-        do ++b;
-        while (b < p.B - 1 && prefix[b + 1] == prefix[b]);
-        if (b < p.B) U = prefix[b + 1] - prefix[b], len = s_len[b];
-      }
-    }
+    if (++u == U) next_pair(b, hk, u, U, len);
   }
   // after a wait that gave up: let the copies in flight land before the CTA's memory is released
   for (; j < nj; ++j) wait_tile(&full[j % SLOTS], (j / SLOTS) & 1);
@@ -710,10 +717,10 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
   __shared__ int s_sum[2][MW];
   pdl_trigger();
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // units before sequence b, and of all; from the lengths, which decode_k has waited for before it let this grid start
+  // cells before sequence b, and of all; from the lengths, which decode_k has waited for before it let this grid start
   int first = 0, all = 0;
   for (int i = threadIdx.x; i < p.B; i += MW * 32) {
-    const int n = units(p, i);
+    const int n = cells(units(p, i));
     first += i < b ? n : 0;
     all += n;
   }
@@ -731,7 +738,7 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
     for (int i = threadIdx.x; i < p.G * D / 8; i += MW * 32) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const int x0 = first * p.Hkv + hk * U, r0 = rg.of(x0), r1 = rg.of(x0 + U - 1);  // ranges of its first and last unit
+  const int x0 = first * p.Hkv + hk * (2 * U + 1) + 1, r0 = rg.of(x0), r1 = rg.of(x0 + 2 * (U - 1));  // ranges of its first and last unit
   if (r0 == r1) return;  // finished by its warp
   const int stripes = p.G >= MW ? 1 : MW / p.G, stripe = warp / p.G;  // (a head and a stripe) per warp, heads in turn if G > MW
   if (stripes == 1 && stripe > 0) return;
@@ -897,7 +904,7 @@ at::Tensor paged_decode_attn_fp8(const at::Tensor& q_, const at::Tensor& k, cons
   AX_CHECK(B <= MAXB, "decode batch must be <= ", MAXB);
   const long rows = c.pages * c.Hkv * c.P;
   AX_CHECK(rows < (1L << 31), "fp8 cache: pages * Hkv * page size must be below 2^31");
-  AX_CHECK(B * (block_table.size(1) * c.P / UNIT + 1) * c.Hkv < (1L << 31), "block_table: too many tokens");
+  AX_CHECK(B * (2 * (block_table.size(1) * c.P / UNIT + 1) + 1) * c.Hkv < (1L << 30), "block_table: too many tokens");
   auto out = at::empty_like(q);
   if (B == 0) return out;
   if (rows == 0 || block_table.size(1) == 0) return out.zero_();
