@@ -237,8 +237,9 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // Work: unit = 64 tokens of one (sequence, kv head).  The units of all (sequence, kv head) pairs in a row form
 // one list, cut into contiguous ranges of equal cost, one per warp of the grid (one CTA per SM): every warp is busy equally
 // long whatever the lengths are.  A pair that lies inside one range is finished by its warp; the others leave fp32
-// partials (at most two per warp), which merge_k combines.  A warp works alone: its own ring of 8 KB slots (K and V tiles
-// in turn) filled by its own TMA loads (128-byte swizzle), no barrier with other warps.
+// partials (at most two per warp), joined first by the CTA, whose ranges are neighbours, and where a pair lies in several
+// CTAs then by merge_k.  While it streams a warp works alone: its own ring of 8 KB slots (K and V tiles in turn) filled
+// by its own TMA loads (128-byte swizzle), no barrier with other warps.
 //
 // Both products are m16n8k16 with f16 operands and fp32 sums; f16 holds every e4m3 code exactly:
 //   S^T (tokens x heads) = Kc Q^T,   O^T (dims x heads) += Vc^T P^T
@@ -298,12 +299,9 @@ struct Ranges {
   }
   __device__ int lo(int r) const { return r * len; }
   __device__ int of(int x) const { return x / len; }
+  __device__ int per_cta(int ctas) const { return max((n + ctas - 1) / ctas, 1); }  // few units still use every SM
 };
 __device__ __forceinline__ int cells(int units) { return units > 0 ? 2 * units + 1 : 0; }
-
-__device__ __forceinline__ int units(const DecParams& p, int b) {
-  return (int)((min((long)max(p.lens[b], 0), (long)p.max_pages * p.P) + UNIT - 1) / UNIT);
-}
 
 // Not volatile: the products may move behind later ldmatrix loads, which keep their order.
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -349,6 +347,78 @@ struct Loader {
   int page;              // its page, fetched ahead; -1: nothing to load
 };
 
+struct Partial {  // of one head: lane l holds dims 4 l .. 4 l + 3
+  float4 o;
+  float m, l;
+};
+__device__ __forceinline__ Partial empty_partial() { return {make_float4(0, 0, 0, 0), -INFINITY, 0.f}; }
+__device__ __forceinline__ Partial load_partial(const DecParams& p, int record, int lane) {
+  const float2 ml = __ldcg(p.part_ml + record);
+  return {__ldcg(reinterpret_cast<const float4*>(p.part_o + (long)record * D + 4 * lane)), ml.x, ml.y};
+}
+// The sum of N partials in the scale of the largest.
+template <int N>
+__device__ __forceinline__ Partial join(const Partial (&x)[N]) {
+  Partial r = empty_partial();
+#pragma unroll
+  for (int k = 0; k < N; ++k) r.m = fmaxf(r.m, x[k].m);
+  const float ref = r.m == -INFINITY ? 0.f : r.m;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float f = ex2(x[k].m - ref);
+    r.l = fmaf(f, x[k].l, r.l);
+    r.o.x = fmaf(f, x[k].o.x, r.o.x), r.o.y = fmaf(f, x[k].o.y, r.o.y), r.o.z = fmaf(f, x[k].o.z, r.o.z), r.o.w = fmaf(f, x[k].o.w, r.o.w);
+  }
+  return r;
+}
+__device__ __forceinline__ void store_output(bf16* dst, const Partial& x, int lane) {
+  const float rl = x.l == 0.f ? 0.f : 1.f / x.l;
+  *reinterpret_cast<bf162*>(dst + 4 * lane) = __floats2bfloat162_rn(x.o.x * rl, x.o.y * rl);
+  *reinterpret_cast<bf162*>(dst + 4 * lane + 2) = __floats2bfloat162_rn(x.o.z * rl, x.o.w * rl);
+}
+
+// Cells of a kv head of the sequences before each (prefix[B]: of all), by all THREADS of the CTA; s_len: the lengths, where wanted.
+template <int THREADS>
+__device__ __forceinline__ void cell_prefix(const DecParams& p, int* prefix, int* s_len, int* s_warp) {
+  const int per = (p.B + THREADS - 1) / THREADS, b0 = threadIdx.x * per, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int sum = 0;
+  for (int i = b0; i < min(b0 + per, p.B); ++i) {
+    const int n = (int)min((long)max(p.lens[i], 0), (long)p.max_pages * p.P);
+    if (s_len != nullptr) s_len[i] = n;
+    prefix[i] = cells((n + UNIT - 1) / UNIT);
+    sum += prefix[i];
+  }
+  int x = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  int before = x - sum;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) before += w < warp ? s_warp[w] : 0;
+  for (int i = b0; i < min(b0 + per, p.B); ++i) {
+    const int n = prefix[i];
+    prefix[i] = before;
+    before += n;
+  }
+  if (threadIdx.x == THREADS - 1) prefix[p.B] = before;
+  __syncthreads();
+}
+// The sequence whose cells of a kv head hold `pos`: the last b with prefix[b] <= pos.  All lanes of a warp.
+__device__ __forceinline__ int sequence_of(const int* prefix, int B, int pos, int lane) {
+  int lo = 0, n = B;  // b in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) >> 5, at = lo + lane * step;
+    const int k = 31 - __clz(__ballot_sync(0xffffffffu, at < lo + n && prefix[min(at, B)] <= pos));
+    n = min(step, lo + n - (lo + k * step));
+    lo += k * step;
+  }
+  return lo;
+}
+
 // 192 registers a thread leave room for a CTA of merge_k on every SM, which waits there for this grid to end.
 template <int NT>
 __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, DecParams p) {
@@ -362,7 +432,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   char* sq = sm + NW * SLOTS * (TILE + UNIT + 12) + warp * Q_BYTES;  // q rows of the pair that is loaded next
   int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12) + NW * Q_BYTES);  // cells of a kv head of the sequences before
   int* s_len = prefix + MAXB + 1;
-  __shared__ int s_warp[NW];
+  __shared__ int s_warp[NW], s_tail[NW], s_pair[NW];
 
   if (lane == 0) {
     for (int s = 0; s < SLOTS; ++s) tc::mbar_init(&full[s], UNIT / p.box);  // every loading lane arrives
@@ -379,56 +449,10 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   }
   pdl_wait();
   pdl_trigger();  // after the wait: merge_k reads the lengths before this grid ends
-  {
-    const int per = (p.B + NW * 32 - 1) / (NW * 32), b0 = threadIdx.x * per;
-    int sum = 0;
-    for (int i = b0; i < min(b0 + per, p.B); ++i) {
-      const int n = (int)min((long)max(p.lens[i], 0), (long)p.max_pages * p.P);
-      s_len[i] = n;
-      sum += cells((n + UNIT - 1) / UNIT);
-    }
-    int x = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) s_warp[warp] = x;
-    __syncthreads();
-    int before = x - sum;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) before += w < warp ? s_warp[w] : 0;
-    for (int i = b0; i < min(b0 + per, p.B); ++i) {
-      prefix[i] = before;
-      before += cells((s_len[i] + UNIT - 1) / UNIT);
-    }
-    if (threadIdx.x == NW * 32 - 1) prefix[p.B] = before;
-    __syncthreads();
-  }
+  cell_prefix<NW * 32>(p, prefix, s_len, s_warp);
   const Ranges rg(prefix[p.B] * p.Hkv, gridDim.x * NW);
-  const int r = warp * gridDim.x + blockIdx.x;  // neighbouring ranges on different SMs: few units still use every SM
-  if (r >= rg.n) return;
-  const int x0 = rg.lo(r);
-
-  int b, hk, u, U, len, left;  // unit that is worked on next, cells of the range from its start on
-  {
-    const int pos = x0 / p.Hkv;  // sequence b: prefix[b] <= pos < prefix[b + 1]
-    int lo = 0, n = p.B;  // b in [lo, lo + n)
-    while (n > 1) {
-      const int step = (n + 31) >> 5, at = lo + lane * step;
-      const int k = 31 - __clz(__ballot_sync(0xffffffffu, at < lo + n && prefix[min(at, p.B)] <= pos));
-      n = min(step, lo + n - (lo + k * step));
-      lo += k * step;
-    }
-    b = lo;
-    const int pc = prefix[b + 1] - prefix[b], rem = x0 - prefix[b] * p.Hkv;
-    U = pc / 2;
-    hk = rem / pc;
-    const int off = rem - hk * pc;
-    u = off / 2;
-    left = min(rg.lo(r + 1), prefix[p.B] * p.Hkv) - x0 - (1 + 2 * u - off);
-    len = s_len[b];
-  }
+  const int wpc = rg.per_cta(gridDim.x), r = blockIdx.x * wpc + warp;
+  int b = 0, hk = 0, u = 0, U = 0, len = 0, left = 0;  // unit that is worked on next, cells of the range from its start on
   auto next_pair = [&](int& b, int& hk, int& u, int& U, int& len) {
     u = 0;
     if (++hk < p.Hkv) return;
@@ -437,11 +461,21 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
     while (b < p.B - 1 && prefix[b + 1] == prefix[b]);
     if (b < p.B) U = (prefix[b + 1] - prefix[b]) / 2, len = s_len[b];
   };
-  if (u == U) {  // the range starts in the second half of the last unit of a pair
-    next_pair(b, hk, u, U, len);
-    left -= 1;  // its own cell; the start of a unit U had been counted already
+  if (warp < wpc && r < rg.n) {
+    const int x0 = rg.lo(r);
+    b = sequence_of(prefix, p.B, x0 / p.Hkv, lane);
+    const int pc = prefix[b + 1] - prefix[b], rem = x0 - prefix[b] * p.Hkv;
+    U = pc / 2;
+    hk = rem / pc;
+    const int off = rem - hk * pc;
+    u = off / 2;
+    left = min(rg.lo(r + 1), prefix[p.B] * p.Hkv) - x0 - (1 + 2 * u - off);
+    len = s_len[b];
+    if (u == U) {  // the range starts in the second half of the last unit of a pair
+      next_pair(b, hk, u, U, len);
+      left -= 1;  // its own cell; the start of a unit U had been counted already
+    }
   }
-  if (left <= 0) return;
   // lane `ch` < chunks loads the box of tokens [ch box, (ch + 1) box) of a unit
   const int chunks = UNIT / p.box;
   const bool loads = lane < chunks;
@@ -466,7 +500,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   };
   const unsigned t0 = (unsigned)u * UNIT + lane * p.box;
   Loader ld{b, hk, u, U, len, left, (int)(t0 / (unsigned)p.P), (int)(t0 % (unsigned)p.P), -1};
-  fetch_page(ld);
+  if (left > 0) fetch_page(ld);
   int nj = 0, row = -1;     // next tile to load (even: K, odd: V of the same unit), its cache row
   bool new_pair = true;     // of `ld`: its q rows come with its K tile
   auto load_next = [&] {
@@ -511,7 +545,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   float acc[NT][8][4], m[NT][2], l[NT][2], qs[NT][2];  // columns 2c, 2c + 1 of a tile: heads 8 t + 2 c, + 1
   uint32_t qf[NT][16];
   bool fresh = true, begun_before = u > 0;  // the pair at the start of the range may have begun in an earlier one
-  int j = 0;
+  int j = 0, tail = 0;  // the pair that goes on in the next range: 1 if it began before this one, 2 if in it
   while (left > 0) {
     const int sk = j % SLOTS, sv = (j + 1) % SLOTS;
     // --- scores of 64 tokens
@@ -696,6 +730,10 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
             if (!whole && g == 0) p.part_ml[slot + h] = make_float2(m[t][cc], sum);
           }
         }
+      if (!ends) {
+        tail = begun_before ? 1 : 2;
+        if (lane == 0) s_pair[warp] = b * p.Hkv + hk;
+      }
       fresh = true;
       begun_before = false;
     }
@@ -703,88 +741,89 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   }
   // after a wait that gave up: let the copies in flight land before the CTA's memory is released
   for (; j < nj; ++j) wait_tile(&full[j % SLOTS], (j / SLOTS) & 1);
+
+  // join the partials of pairs that lie in several ranges of this CTA: the chain of a warp whose pair goes on
+  if (lane == 0) s_tail[warp] = tail;
+  __syncthreads();
+  for (int task = warp; task < (wpc - 1) * p.G; task += NW) {
+    const int a = task / p.G, h = task - a * p.G;
+    if (!(s_tail[a] == 2 || (a == 0 && s_tail[a] == 1))) continue;  // no pair goes on, or its chain starts at an earlier warp
+    int z = a + 1;
+    while (s_tail[z] == 1 && z < wpc - 1) ++z;
+    const int ra = blockIdx.x * wpc, first = ((ra + a) * 2 + (s_tail[a] == 2)) * p.G + h;
+    Partial x[NW];
+#pragma unroll
+    for (int k = 0; k < NW; ++k) x[k] = a + k <= z ? load_partial(p, k == 0 ? first : (ra + a + k) * 2 * p.G + h, lane) : empty_partial();
+    const Partial y = join(x);
+    if (s_tail[a] == 2 && s_tail[z] != 1) {  // began and ended here
+      const int pair = s_pair[a];
+      store_output(p.out + ((long)pair * p.G + h) * D, y, lane);
+    } else {
+      *reinterpret_cast<float4*>(p.part_o + (long)first * D + 4 * lane) = y.o;
+      if (lane == 0) p.part_ml[first] = make_float2(y.m, y.l);
+    }
+  }
 }
 
-// The pairs that more than one range holds: out = sum_r 2^{m_r - M} o_r / sum_r 2^{m_r - M} l_r; zeros for empty sequences.
-// One CTA per (sequence, kv head).  Its MW warps are dealt to the heads of the group and, where those are fewer, to
-// stripes of the partials, whose loads are all in flight at once (a long context has up to 2 x 74 of them on 16 pairs: one
-// warp walking them took 42 us, stripes 3).
+// The pairs that lie in several CTAs of decode_k (at most one begins in each and goes on): out = the joined partials of
+// those CTAs; zeros for empty sequences.  CTA i looks for the pair that goes on behind CTA i before decode_k has ended; then
+// its MW warps are dealt to the heads of the group and, where those are fewer, to stripes of the partials, whose loads
+// are all in flight at once.  One warp walking the partials of all warps took 42 us for two contexts of 100k, CTAs of
+// eight warps for every pair 6 us, and 5 us for 256 short sequences; this form TODO.
 constexpr int MW = 8, MBATCH = 4;
 
 __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
-  __shared__ float s_o[MW][D];
+  __shared__ int prefix[MAXB + 1], s_warp[MW];
+  __shared__ float4 s_o[MW][32];
   __shared__ float2 s_ml[MW];
-  __shared__ int s_sum[2][MW];
   pdl_trigger();
-  const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // cells before sequence b, and of all; from the lengths, which decode_k has waited for before it let this grid start
-  int first = 0, all = 0;
-  for (int i = threadIdx.x; i < p.B; i += MW * 32) {
-    const int n = cells(units(p, i));
-    first += i < b ? n : 0;
-    all += n;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  cell_prefix<MW * 32>(p, prefix, nullptr, s_warp);  // decode_k lets this grid start only once the lengths are there
+  const Ranges rg(prefix[p.B] * p.Hkv, p.ranges);
+  const int wpc = rg.per_cta(gridDim.x), end = min(rg.lo((blockIdx.x + 1) * wpc), prefix[p.B] * p.Hkv);  // of CTA i's cells
+  int r0 = 0, r1 = -1;  // ranges of the first and last unit of the pair that goes on
+  bf16* out = nullptr;
+  if (end > 0 && end < prefix[p.B] * p.Hkv) {
+    const int b = sequence_of(prefix, p.B, (end - 1) / p.Hkv, lane), pc = prefix[b + 1] - prefix[b];
+    const int hk = (end - 1 - prefix[b] * p.Hkv) / pc, x0 = prefix[b] * p.Hkv + hk * pc + 1, last = x0 + pc - 3;
+    if (x0 < end && last >= end && rg.of(x0) >= (int)blockIdx.x * wpc) {
+      r0 = rg.of(x0), r1 = rg.of(last);
+      out = p.out + ((long)b * p.Hkv + hk) * p.G * D;
+    }
   }
-  first = __reduce_add_sync(0xffffffffu, first), all = __reduce_add_sync(0xffffffffu, all);
-  if (lane == 0) s_sum[0][warp] = first, s_sum[1][warp] = all;
-  __syncthreads();
-  first = all = 0;
-#pragma unroll
-  for (int w = 0; w < MW; ++w) first += s_sum[0][w], all += s_sum[1][w];
-  const int U = units(p, b);
-  const Ranges rg(all * p.Hkv, p.ranges);
   pdl_wait();
-  bf16* out = p.out + ((long)b * p.Hkv + hk) * p.G * D;
-  if (U == 0) {
-    for (int i = threadIdx.x; i < p.G * D / 8; i += MW * 32) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const int x0 = first * p.Hkv + hk * (2 * U + 1) + 1, r0 = rg.of(x0), r1 = rg.of(x0 + 2 * (U - 1));  // ranges of its first and last unit
-  if (r0 == r1) return;  // finished by its warp
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x)
+    if (prefix[b + 1] == prefix[b])
+      for (int i = threadIdx.x; i < p.Hkv * p.G * D / 8; i += MW * 32) reinterpret_cast<uint4*>(p.out + (long)b * p.Hkv * p.G * D)[i] = make_uint4(0, 0, 0, 0);
+  if (out == nullptr) return;
+  const int n = r1 / wpc - (int)blockIdx.x + 1;  // CTAs that the pair lies in
   const int stripes = p.G >= MW ? 1 : MW / p.G, stripe = warp / p.G;  // (a head and a stripe) per warp, heads in turn if G > MW
   if (stripes == 1 && stripe > 0) return;
   for (int h = warp % p.G; h < p.G; h += MW) {
-    float M = -INFINITY, L = 0.f;
-    float4 o = make_float4(0, 0, 0, 0);
+    Partial y = empty_partial();
     if (stripe < stripes)
-      for (int r = r0 + stripe; r <= r1; r += stripes * MBATCH) {
-        float2 ml[MBATCH];
-        float4 v[MBATCH];
-        float mx = M;
+      for (int k = stripe; k < n; k += stripes * MBATCH) {
+        Partial x[MBATCH + 1];
 #pragma unroll
-        for (int k = 0; k < MBATCH; ++k) {
-          const int rk = r + k * stripes, i = (rk * 2 + (rk == r0 ? 1 : 0)) * p.G + h;  // the pair starts in its first range: slot 1
-          ml[k] = rk <= r1 ? p.part_ml[i] : make_float2(-INFINITY, 0.f);
-          v[k] = rk <= r1 ? *reinterpret_cast<const float4*>(p.part_o + (long)i * D + 4 * lane) : make_float4(0, 0, 0, 0);
-          mx = fmaxf(mx, ml[k].x);
+        for (int i = 0; i < MBATCH; ++i) {
+          const int at = k + i * stripes;
+          x[i] = at < n ? load_partial(p, (at == 0 ? r0 * 2 + 1 : ((int)blockIdx.x + at) * wpc * 2) * p.G + h, lane) : empty_partial();
         }
-        const float ref = mx == -INFINITY ? 0.f : mx, a = ex2(M - ref);
-        M = mx;
-        L *= a, o.x *= a, o.y *= a, o.z *= a, o.w *= a;
-#pragma unroll
-        for (int k = 0; k < MBATCH; ++k) {
-          const float f = ex2(ml[k].x - ref);
-          L = fmaf(f, ml[k].y, L);
-          o.x = fmaf(f, v[k].x, o.x), o.y = fmaf(f, v[k].y, o.y), o.z = fmaf(f, v[k].z, o.z), o.w = fmaf(f, v[k].w, o.w);
-        }
+        x[MBATCH] = y;
+        y = join(x);
       }
     if (stripes > 1) {
-      *reinterpret_cast<float4*>(&s_o[warp][4 * lane]) = o;
-      if (lane == 0) s_ml[warp] = make_float2(M, L);
+      s_o[warp][lane] = y.o;
+      if (lane == 0) s_ml[warp] = make_float2(y.m, y.l);
       __syncthreads();  // G < MW: every warp passes here once
       if (stripe > 0) return;
       for (int k = 1; k < stripes; ++k) {
         const float2 ml = s_ml[warp + k * p.G];
-        const float4 v = *reinterpret_cast<const float4*>(&s_o[warp + k * p.G][4 * lane]);
-        const float mx = fmaxf(M, ml.x), ref = mx == -INFINITY ? 0.f : mx, a = ex2(M - ref), f = ex2(ml.x - ref);
-        M = mx;
-        L = fmaf(f, ml.y, L * a);
-        o.x = fmaf(f, v.x, o.x * a), o.y = fmaf(f, v.y, o.y * a), o.z = fmaf(f, v.z, o.z * a), o.w = fmaf(f, v.w, o.w * a);
+        const Partial x[2] = {y, {s_o[warp + k * p.G][lane], ml.x, ml.y}};
+        y = join(x);
       }
     }
-    const float rl = L == 0.f ? 0.f : 1.f / L;
-    bf16* dst = out + h * D + 4 * lane;
-    *reinterpret_cast<bf162*>(dst) = __floats2bfloat162_rn(o.x * rl, o.y * rl);
-    *reinterpret_cast<bf162*>(dst + 2) = __floats2bfloat162_rn(o.z * rl, o.w * rl);
+    store_output(out + h * D, y, lane);
   }
 }
 
@@ -922,7 +961,7 @@ at::Tensor paged_decode_attn_fp8(const at::Tensor& q_, const at::Tensor& k, cons
   smem_attr((const void*)kern, DEC_SMEM);
   launch_pdl(kern, dim3(grid), dim3(NW * 32), DEC_SMEM, stream(), tk, tv, p);
   AX_LAUNCH_OK();
-  launch_pdl(merge_k, dim3((unsigned)(B * c.Hkv)), dim3(MW * 32), 0, stream(), p);
+  launch_pdl(merge_k, dim3(grid), dim3(MW * 32), 0, stream(), p);
   AX_LAUNCH_OK();
   return out;
 }
