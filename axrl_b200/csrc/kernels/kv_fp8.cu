@@ -237,9 +237,9 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // Work: unit = 64 tokens of one (sequence, kv head).  The units of all (sequence, kv head) pairs in a row form
 // one list, cut into contiguous ranges of equal cost, one per warp of the grid (one CTA per SM): every warp is busy equally
 // long whatever the lengths are.  A pair that lies inside one range is finished by its warp; the others leave fp32
-// partials (at most two per warp), joined first by the CTA, whose ranges are neighbours, and where a pair lies in several
-// CTAs then by merge_k.  While it streams a warp works alone: its own ring of 8 KB slots (K and V tiles in turn) filled
-// by its own TMA loads (128-byte swizzle), no barrier with other warps.
+// partials in shared memory (at most two per warp), which the CTA, whose ranges are neighbours, joins at its end; what then
+// lies in several CTAs (at most two partials each) is joined by merge_k.  While it streams a warp works alone: its own ring of
+// 8 KB slots (K and V tiles in turn) filled by its own TMA loads (128-byte swizzle), no barrier with other warps.
 //
 // Both products are m16n8k16 with f16 operands and fp32 sums; f16 holds every e4m3 code exactly:
 //   S^T (tokens x heads) = Kc Q^T,   O^T (dims x heads) += Vc^T P^T
@@ -258,8 +258,12 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // two so that their largest is in [2^14, 2^15) and round to f16 exactly but for what is below 2^-28 of it.
 constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 2, TILE = UNIT * D;  // TILE: bytes of one slot
 constexpr int MAXB = 2048;
-constexpr int Q_BYTES = MAXG * D * 2;  // q rows of a pair
-constexpr int DEC_SMEM = 1024 + NW * SLOTS * (TILE + UNIT + 8 + 4) + NW * Q_BYTES + (2 * MAXB + 1) * 4;
+constexpr int DEC_FIXED = NW * SLOTS * (TILE + UNIT + 8 + 4);
+// Shared memory of a CTA: rings, scales, barriers, flags; q rows, partials of pairs that began before the warps' ranges (groups of
+// up to eight heads; larger ones keep them in global memory meanwhile), their maxima and sums; cell prefix and lengths.
+constexpr int dec_smem(int G, int B) { return 1024 + DEC_FIXED + NW * G * (D * 2 + (G <= 8 ? D * 4 : 0) + 16) + (2 * B + 1) * 4; }
+static_assert(dec_smem(8, MAXB) <= 227 * 1024 - 256 && dec_smem(MAXG, MAXB) <= 227 * 1024 - 256, "shared memory");
+static_assert(2 * MAXG * D * 4 <= SLOTS * TILE, "both partials of a warp fit its ring");
 
 __device__ int g_decode_err;  // first wait that gave up (0: none)
 
@@ -269,8 +273,9 @@ struct DecParams {
   const int* lens;     // (B,)
   const uint8_t *ks, *vs;
   bf16* out;           // (B, Hq, 128)
-  float* part_o;       // (ranges, 2, G, 128)
-  float2* part_ml;     // (ranges, 2, G): max, sum
+  float* part_o;       // (CTAs, 2, G, 128): of the pair that began before the CTA's ranges, of the one that goes on behind them
+  float2* part_ml;     // (CTAs, 2, G): max, sum
+  float* part_w;       // (CTAs, NW, G, 128), groups above eight: kept for the warps' first pairs
   int ranges;          // most ranges: warps of decode_k
   long pages;
   int B, G, Hkv, P, max_pages, box;  // box: token rows of one TMA load, gcd(P, 64)
@@ -429,10 +434,12 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   uint8_t* sc = reinterpret_cast<uint8_t*>(sm + NW * SLOTS * TILE) + warp * SLOTS * UNIT;  // scale bytes of a slot's tokens
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + NW * SLOTS * (TILE + UNIT)) + warp * SLOTS;
   uchar4* meta = reinterpret_cast<uchar4*>(sm + NW * SLOTS * (TILE + UNIT + 8)) + warp * SLOTS;  // which chunks of a slot were loaded
-  char* sq = sm + NW * SLOTS * (TILE + UNIT + 12) + warp * Q_BYTES;  // q rows of the pair that is loaded next
-  int* prefix = reinterpret_cast<int*>(sm + NW * SLOTS * (TILE + UNIT + 12) + NW * Q_BYTES);  // cells of a kv head of the sequences before
-  int* s_len = prefix + MAXB + 1;
-  __shared__ int s_warp[NW], s_tail[NW], s_pair[NW];
+  char* sq = sm + DEC_FIXED + warp * p.G * D * 2;  // q rows of the pair that is loaded next
+  float* s_rec = reinterpret_cast<float*>(sm + DEC_FIXED + NW * p.G * D * 2);
+  float2* s_ml = reinterpret_cast<float2*>(s_rec + (NT == 1 ? NW * p.G * D : 0));  // [warp][began before, goes on][head]
+  int* prefix = reinterpret_cast<int*>(s_ml + NW * 2 * p.G);
+  int* s_len = prefix + p.B + 1;
+  __shared__ int s_warp[NW], s_head[NW], s_tail[NW], s_pair[NW];
 
   if (lane == 0) {
     for (int s = 0; s < SLOTS; ++s) tc::mbar_init(&full[s], UNIT / p.box);  // every loading lane arrives
@@ -545,7 +552,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   float acc[NT][8][4], m[NT][2], l[NT][2], qs[NT][2];  // columns 2c, 2c + 1 of a tile: heads 8 t + 2 c, + 1
   uint32_t qf[NT][16];
   bool fresh = true, begun_before = u > 0;  // the pair at the start of the range may have begun in an earlier one
-  int j = 0, tail = 0;  // the pair that goes on in the next range: 1 if it began before this one, 2 if in it
+  int j = 0, head = 0, tail = 0;  // a pair that began before this range has a partial; the pair that goes on behind it: 1 if it began before, 2 if in it
   while (left > 0) {
     const int sk = j % SLOTS, sv = (j + 1) % SLOTS;
     // --- scores of 64 tokens
@@ -709,7 +716,9 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
     left -= ends ? 3 : 2;
     if (ends || left <= 0) {
       const bool whole = ends && !begun_before;
-      const int slot = (r * 2 + (begun_before ? 0 : 1)) * p.G;
+      // what goes on lies in this warp's ring, whose tiles have all been used by then
+      float* rec = !begun_before ? reinterpret_cast<float*>(ring) : NT == 1 ? s_rec + warp * p.G * D : p.part_w + ((long)blockIdx.x * NW + warp) * p.G * D;
+      float2* rec_ml = s_ml + (warp * 2 + !begun_before) * p.G;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -721,15 +730,16 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
           if (h < p.G) {
             const float rl = sum == 0.f ? 0.f : 1.f / sum;
             bf16* dst = p.out + (((long)b * p.Hkv + hk) * p.G + h) * D + g;
-            float* part = p.part_o + (long)(slot + h) * D + g;
+            float* part = rec + h * D + g;
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
               if (whole) dst[16 * d] = __float2bfloat16(acc[t][d][cc] * rl), dst[16 * d + 8] = __float2bfloat16(acc[t][d][2 + cc] * rl);
               else part[16 * d] = acc[t][d][cc], part[16 * d + 8] = acc[t][d][2 + cc];
             }
-            if (!whole && g == 0) p.part_ml[slot + h] = make_float2(m[t][cc], sum);
+            if (!whole && g == 0) rec_ml[h] = make_float2(m[t][cc], sum);
           }
         }
+      head |= begun_before;
       if (!ends) {
         tail = begun_before ? 1 : 2;
         if (lane == 0) s_pair[warp] = b * p.Hkv + hk;
@@ -742,26 +752,44 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   // after a wait that gave up: let the copies in flight land before the CTA's memory is released
   for (; j < nj; ++j) wait_tile(&full[j % SLOTS], (j / SLOTS) & 1);
 
-  // join the partials of pairs that lie in several ranges of this CTA: the chain of a warp whose pair goes on
-  if (lane == 0) s_tail[warp] = tail;
+  // Join the partials of pairs that lie in several ranges of this CTA: a warp takes a head and walks the ranges in order.
+  if (NT == 2 && head) {
+    __syncwarp();
+    const float4* from = reinterpret_cast<const float4*>(p.part_w + ((long)blockIdx.x * NW + warp) * p.G * D);
+    float4* to = reinterpret_cast<float4*>(ring) + p.G * 32;
+    for (int i = lane; i < p.G * 32; i += 32) to[i] = __ldcg(from + i);
+  }
+  if (lane == 0) s_head[warp] = head, s_tail[warp] = tail;
   __syncthreads();
-  for (int task = warp; task < (wpc - 1) * p.G; task += NW) {
-    const int a = task / p.G, h = task - a * p.G;
-    if (!(s_tail[a] == 2 || (a == 0 && s_tail[a] == 1))) continue;  // no pair goes on, or its chain starts at an earlier warp
-    int z = a + 1;
-    while (s_tail[z] == 1 && z < wpc - 1) ++z;
-    const int ra = blockIdx.x * wpc, first = ((ra + a) * 2 + (s_tail[a] == 2)) * p.G + h;
-    Partial x[NW];
-#pragma unroll
-    for (int k = 0; k < NW; ++k) x[k] = a + k <= z ? load_partial(p, k == 0 ? first : (ra + a + k) * 2 * p.G + h, lane) : empty_partial();
-    const Partial y = join(x);
-    if (s_tail[a] == 2 && s_tail[z] != 1) {  // began and ended here
-      const int pair = s_pair[a];
-      store_output(p.out + ((long)pair * p.G + h) * D, y, lane);
-    } else {
-      *reinterpret_cast<float4*>(p.part_o + (long)first * D + 4 * lane) = y.o;
-      if (lane == 0) p.part_ml[first] = make_float2(y.m, y.l);
+  for (int h = warp; h < p.G; h += NW) {
+    Partial y = empty_partial();
+    int pair = -1, open = 0;  // the pair of y if it began in this CTA; y holds something
+    auto record = [&](int w, int which) -> Partial {
+      const char* ring_w = sm + w * SLOTS * TILE;
+      const float4* rec = reinterpret_cast<const float4*>(which ? ring_w : NT == 1 ? reinterpret_cast<const char*>(s_rec + w * p.G * D) : ring_w + p.G * D * 4);
+      const float2 ml = s_ml[(w * 2 + which) * p.G + h];
+      return {rec[h * 32 + lane], ml.x, ml.y};
+    };
+    auto hand_on = [&](int which) {
+      const int at = (blockIdx.x * 2 + which) * p.G + h;
+      *reinterpret_cast<float4*>(p.part_o + (long)at * D + 4 * lane) = y.o;
+      if (lane == 0) p.part_ml[at] = make_float2(y.m, y.l);
+    };
+#pragma unroll 1
+    for (int w = 0; w < wpc; ++w) {
+      if (s_head[w]) {
+        const Partial two[2] = {y, record(w, 0)};
+        y = join(two);
+        open = 1;
+        if (s_tail[w] != 1) {  // ends here
+          if (pair >= 0) store_output(p.out + ((long)pair * p.G + h) * D, y, lane);
+          else hand_on(0);
+          y = empty_partial(), open = 0, pair = -1;
+        }
+      }
+      if (s_tail[w] == 2) y = record(w, 1), open = 1, pair = s_pair[w];
     }
+    if (open) hand_on(pair >= 0 ? 1 : 0);
   }
 }
 
@@ -773,7 +801,8 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
 constexpr int MW = 8, MBATCH = 4;
 
 __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
-  __shared__ int prefix[MAXB + 1], s_warp[MW];
+  extern __shared__ int prefix[];
+  __shared__ int s_warp[MW];
   __shared__ float4 s_o[MW][32];
   __shared__ float2 s_ml[MW];
   pdl_trigger();
@@ -781,13 +810,13 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
   cell_prefix<MW * 32>(p, prefix, nullptr, s_warp);  // decode_k lets this grid start only once the lengths are there
   const Ranges rg(prefix[p.B] * p.Hkv, p.ranges);
   const int wpc = rg.per_cta(gridDim.x), end = min(rg.lo((blockIdx.x + 1) * wpc), prefix[p.B] * p.Hkv);  // of CTA i's cells
-  int r0 = 0, r1 = -1;  // ranges of the first and last unit of the pair that goes on
+  int n = 0;  // CTAs that the pair that goes on lies in
   bf16* out = nullptr;
   if (end > 0 && end < prefix[p.B] * p.Hkv) {
     const int b = sequence_of(prefix, p.B, (end - 1) / p.Hkv, lane), pc = prefix[b + 1] - prefix[b];
     const int hk = (end - 1 - prefix[b] * p.Hkv) / pc, x0 = prefix[b] * p.Hkv + hk * pc + 1, last = x0 + pc - 3;
     if (x0 < end && last >= end && rg.of(x0) >= (int)blockIdx.x * wpc) {
-      r0 = rg.of(x0), r1 = rg.of(last);
+      n = rg.of(last) / wpc - (int)blockIdx.x + 1;
       out = p.out + ((long)b * p.Hkv + hk) * p.G * D;
     }
   }
@@ -796,7 +825,6 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
     if (prefix[b + 1] == prefix[b])
       for (int i = threadIdx.x; i < p.Hkv * p.G * D / 8; i += MW * 32) reinterpret_cast<uint4*>(p.out + (long)b * p.Hkv * p.G * D)[i] = make_uint4(0, 0, 0, 0);
   if (out == nullptr) return;
-  const int n = r1 / wpc - (int)blockIdx.x + 1;  // CTAs that the pair lies in
   const int stripes = p.G >= MW ? 1 : MW / p.G, stripe = warp / p.G;  // (a head and a stripe) per warp, heads in turn if G > MW
   if (stripes == 1 && stripe > 0) return;
   for (int h = warp % p.G; h < p.G; h += MW) {
@@ -807,7 +835,7 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
 #pragma unroll
         for (int i = 0; i < MBATCH; ++i) {
           const int at = k + i * stripes;
-          x[i] = at < n ? load_partial(p, (at == 0 ? r0 * 2 + 1 : ((int)blockIdx.x + at) * wpc * 2) * p.G + h, lane) : empty_partial();
+          x[i] = at < n ? load_partial(p, (((int)blockIdx.x + at) * 2 + (at == 0)) * p.G + h, lane) : empty_partial();
         }
         x[MBATCH] = y;
         y = join(x);
@@ -949,19 +977,20 @@ at::Tensor paged_decode_attn_fp8(const at::Tensor& q_, const at::Tensor& k, cons
   if (rows == 0 || block_table.size(1) == 0) return out.zero_();
   const int G = (int)(Hq / c.Hkv), grid = num_sms(), ranges = grid * NW;
   // partials: freed after the launches, so the memory is handed on in stream order (and is the graph's when captured)
-  const long floats = (long)ranges * 2 * G * D;
-  const c10::DataPtr part = c10::cuda::CUDACachingAllocator::get()->allocate((floats + (long)ranges * 2 * G * 2) * sizeof(float));
+  const long joined = (long)grid * 2 * G, kept = G <= 8 ? 0 : (long)grid * NW * G;
+  const c10::DataPtr part = c10::cuda::CUDACachingAllocator::get()->allocate((joined * (D + 2) + kept * D) * sizeof(float));
+  float* part_o = (float*)part.get();
   int box = 16;
   while (box < 64 && c.P % (2 * box) == 0) box *= 2;
   const CUtensorMap tk = codes_map(c.k, rows, box), tv = codes_map(c.v, rows, box);
   const DecParams p{(const bf16*)q.data_ptr(), (const int*)block_table.data_ptr(), (const int*)seq_lens.data_ptr(), c.ks, c.vs, (bf16*)out.data_ptr(),
-                    (float*)part.get(), (float2*)((float*)part.get() + floats), ranges, c.pages, (int)B, G, c.Hkv, c.P,
+                    part_o, (float2*)(part_o + joined * D), part_o + joined * (D + 2), ranges, c.pages, (int)B, G, c.Hkv, c.P,
                     (int)block_table.size(1), box, (float)(scale * 1.4426950408889634)};
   auto kern = G <= 8 ? decode_k<1> : decode_k<2>;
-  smem_attr((const void*)kern, DEC_SMEM);
-  launch_pdl(kern, dim3(grid), dim3(NW * 32), DEC_SMEM, stream(), tk, tv, p);
+  smem_attr((const void*)kern, 227 * 1024 - 256);
+  launch_pdl(kern, dim3(grid), dim3(NW * 32), dec_smem(G, (int)B), stream(), tk, tv, p);
   AX_LAUNCH_OK();
-  launch_pdl(merge_k, dim3(grid), dim3(MW * 32), 0, stream(), p);
+  launch_pdl(merge_k, dim3(grid), dim3(MW * 32), (B + 1) * sizeof(int), stream(), p);
   AX_LAUNCH_OK();
   return out;
 }
