@@ -1,6 +1,6 @@
 """Rollout-engine microbenchmark: prefill + decode throughput of a Qwen3-shaped model.
 
-python -m axrl_b200.benchmarks.decode_bench --model qwen3-8b --batch 256 --prompt 512 --new 256 [--pdl 0]
+python -m axrl_b200.benchmarks.decode_bench --model qwen3-8b --batch 256 --prompt 512 --new 256 [--kv fp8_block] [--pdl 0]
 (AXRL_DECODE_GEMM=skinny|tma|tcgen05 forces the decode-size GEMM kernel.)  Reports device-timed prefill seconds, decode ms/step and decode tokens/s (CUDA events).
 """
 
@@ -21,6 +21,7 @@ def main() -> None:
     ap.add_argument("--group", type=int, default=8)
     ap.add_argument("--eager", action="store_true")
     ap.add_argument("--burst", type=int, default=16)
+    ap.add_argument("--kv", default="bf16", choices=["bf16", "fp8_block"], help="KV cache format")
     ap.add_argument("--pdl", type=int, default=1, help="programmatic dependent launch of the decode kernels (0 = off)")
     a = ap.parse_args()
     import os
@@ -39,7 +40,7 @@ def main() -> None:
     model.inv_freq = model.inv_freq.float()
     ctx = a.prompt + a.new + 64
     eng = RolloutEngine(model, max_batch=a.batch, kv_tokens=a.batch * (ctx + 64), max_context=ctx, use_cuda_graph=not a.eager,
-                        burst=a.burst)
+                        burst=a.burst, kv_format=a.kv)
 
     def reqs(tag: str) -> list[GenRequest]:
         g = torch.Generator().manual_seed(0)
@@ -64,7 +65,7 @@ def main() -> None:
                       "prefill_s": round(st["prefill_s"], 3), "decode_s": round(st["decode_s"], 3),
                       "decode_ms_per_step": round(1000 * st["decode_s"] / max(1, st["decode_steps"]), 3),
                       "decode_tok_per_s": round(st["decode_tokens"] / max(1e-9, st["decode_s"]), 1), "bursts": st["bursts"],
-                      "graph": not a.eager, "pdl": bool(a.pdl), "decode_gemm": os.environ.get("AXRL_DECODE_GEMM", "default")}))
+                      "graph": not a.eager, "kv": a.kv, "pdl": bool(a.pdl), "decode_gemm": os.environ.get("AXRL_DECODE_GEMM", "default")}))
     eng.release_graphs()
 
 

@@ -179,7 +179,8 @@ class RolloutWorkerConfig(InferWorkerConfig):
     max_num_batched_tokens: int | None = None
     load_dummy_weights: bool = False
     attention_backend: str | None = None
-    kv_cache_dtype: Literal["auto", "fp8_e4m3", "fp8_e5m2"] = "auto"
+    # "fp8_block" (no reference counterpart): e4m3 pages with one power-of-two scale per (token, head)
+    kv_cache_dtype: Literal["auto", "fp8_e4m3", "fp8_e5m2", "fp8_block"] = "auto"
     prefill_max_requests: int | None = None
     enable_fp32_lm_head: bool = True
     enable_metrics: bool = True
@@ -198,10 +199,10 @@ class RolloutWorkerConfig(InferWorkerConfig):
     @field_validator("kv_cache_dtype")
     @classmethod
     def _kv_dtype_supported(cls, v: str) -> str:
-        # The paged KV cache and its decode kernel are bf16; an fp8 cache would be accepted and
-        # silently stored in bf16, so it is rejected instead.
-        if v != "auto":
-            raise ValueError(f"kv_cache_dtype={v!r} is not supported by the rollout engine (bf16 KV cache only); use 'auto'")
+        # The reference's fp8 types have no scales per token; accepting them and storing something
+        # else would be silent, so they are rejected.
+        if v not in ("auto", "fp8_block"):
+            raise ValueError(f"kv_cache_dtype={v!r} is not supported by the rollout engine; use 'auto' (bf16) or 'fp8_block'")
         return v
 
     def gpus_per_worker(self) -> int:

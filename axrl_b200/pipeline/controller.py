@@ -81,7 +81,8 @@ class PipelineController:
         kv_tokens = int(rw.max_running_requests * (max_ctx + 128))
         self.engine = RolloutEngine(self.train.model, max_batch=rw.max_running_requests, kv_tokens=kv_tokens, page_size=rw.kv_page_size,
                                     max_context=max_ctx, use_cuda_graph=rw.use_cuda_graph, seed=c.megatron_worker.seed,
-                                    dp_attention=_ep_active(self.train.model))
+                                    dp_attention=_ep_active(self.train.model),
+                                    kv_format="fp8_block" if rw.kv_cache_dtype == "fp8_block" else "bf16")
         self.worker = RolloutWorker(self.engine, c.train_sampling_config, continue_after_abort=rw.continue_generation_after_abort)
         self.router = InferenceRouter([self.worker], max_imbalance=rw.max_imbalance)
         self.rollout_queue: AsyncTaskQueue = AsyncTaskQueue(max_running=c.controller.max_running_requests, name="rollout")

@@ -9,6 +9,10 @@ sampled-token logprobs (:489-580), abort-and-continue for partial rollout
 Design (B200-first):
 * KV lives in one tensor ``[L, 2, pages, Hkv, page_size, 128]`` bf16; the C++
   ``BlockManager`` owns page allocation, refcounts and the prefix cache;
+  ``kv_format="fp8_block"`` holds it in e4m3 with one power of two per (token, head) instead
+  (``ops/paged_fp8.py``): half the bytes, and prompts that begin with cached pages prefill only
+  their rest, attending to the prefix rows loaded back from the cache (every reader of a row sees
+  the same values, so the outcome does not depend on who computed the prefix);
 * requests that share a prompt (a GRPO group) are prefilled ONCE; members share
   the prompt's full pages by refcount and copy the partial last page;
 * prefill runs the packed range-list attention over new prompts while the fused
@@ -38,7 +42,7 @@ import torch
 from axrl_b200.models.qwen3 import Qwen3Model
 from axrl_b200.ops import _ext
 from axrl_b200.ops import core as ops
-from axrl_b200.ops import paged
+from axrl_b200.ops import paged, paged_fp8
 from axrl_b200.ops.attention_spec import spec_from_triples
 from axrl_b200.rollout.kv import make_block_manager
 from axrl_b200.utils import iostats
@@ -117,7 +121,7 @@ class RolloutEngine:
                  max_context: int = 16384, max_prefill_tokens: int = 16384, use_cuda_graph: bool = True, seed: int = 0,
                  eos_token_id: int | None = None, burst: int = 16, kv_memory_saver: bool = False, weight_format: str = "bf16",
                  tp_group: Any = None, embed_full: torch.Tensor | None = None, tokenizer: Any = None,
-                 dp_attention: bool = False) -> None:
+                 dp_attention: bool = False, kv_format: str = "bf16") -> None:
         self.model = model
         # data-parallel attention over an expert-parallel model: every EP rank serves its own requests
         # (own KV cache, own batch) and the ranks step in lockstep so each MoE layer's dispatch /
@@ -154,7 +158,25 @@ class RolloutEngine:
         self.num_pages = max(2, math.ceil(kv_tokens / page_size)) + 1  # last page: scratch for frozen/padded rows
         self.scratch_page = self.num_pages - 1
         self.kv_buf = None
-        if self.is_cuda and kv_memory_saver:
+        if kv_format not in ("bf16", "fp8_block"):
+            raise ValueError(f"kv_format={kv_format!r}: 'bf16' or 'fp8_block'")
+        self.kv_format = kv_format
+        self.kv_fp8 = None  # (codes [L, 2, pages, Hkv, P, D], scales [L, 2, pages, Hkv, P])
+        if kv_format == "fp8_block":
+            if self.is_cuda and (D != 128 or page_size % 16 or attn0.nq > 16 * Hkv or max_batch > 2048):
+                raise ValueError("kv_format='fp8_block' needs head_dim 128, pages of a multiple of 16 tokens, GQA groups up to 16 and max_batch up to 2048")
+            if self.is_cuda and kv_memory_saver:
+                from axrl_b200.runtime.vmm import VmmBuffer
+
+                rows = L * 2 * self.num_pages * Hkv * page_size
+                self.kv_buf = VmmBuffer((rows * (D + 1),), torch.uint8, tag=f"kv_cache_{id(self)}")
+                flat = self.kv_buf.tensor
+                self.kv_fp8 = (flat[:rows * D].view(torch.float8_e4m3fn).view(L, 2, self.num_pages, Hkv, page_size, D),
+                               flat[rows * D:].view(torch.float8_e8m0fnu).view(L, 2, self.num_pages, Hkv, page_size))
+            else:
+                self.kv_fp8 = paged_fp8.empty_cache((L,), self.num_pages, Hkv, page_size, self.device, dim=D)
+            self.kv = None
+        elif self.is_cuda and kv_memory_saver:
             # KV pages live in a VMM-tagged region: released while the trainer runs, re-mapped at the
             # same address before the next rollout (captured decode graphs stay valid).
             from axrl_b200.runtime.vmm import VmmBuffer
@@ -166,7 +188,8 @@ class RolloutEngine:
         self.preempted: dict[str, _Seq] = {}
         self.bm = make_block_manager(self.num_pages - 1, page_size)
         self.max_pages = math.ceil(max_context / page_size) + 1
-        self.ws = paged.DecodeWorkspace(max_batch, attn0.nq, max_context + page_size, self.device) if self.is_cuda else None
+        # (the 8-bit decode attention plans for itself)
+        self.ws = paged.DecodeWorkspace(max_batch, attn0.nq, max_context + page_size, self.device) if self.is_cuda and self.kv_fp8 is None else None
         self.use_graph = use_cuda_graph and self.is_cuda and not cfg.is_moe
         self.graphs: dict[int, tuple] = {}
         self.seed = seed
@@ -213,6 +236,8 @@ class RolloutEngine:
         params = dict(self.model.named_parameters())
         for name, (q, s) in weights.items():
             self.fp8[id(params[name])] = Fp8Weight(q, s)
+        if self.kv_fp8 is not None:
+            self.reset_prefix_cache()
 
     # ------------------------------------------------------------------ static buffers
     def _alloc_static(self) -> None:
@@ -288,7 +313,20 @@ class RolloutEngine:
             return _ext.ext().embed_fwd(ids, self.model.embed_tokens)
         return torch.nn.functional.embedding(ids, self.model.embed_tokens)
 
-    def _layers_tp(self, h, pos, slots, attend):  # noqa: ANN001, ANN202
+    def _append_kv(self, li: int, a, qkv: torch.Tensor, pos: torch.Tensor, inv: torch.Tensor, slots: torch.Tensor, want_kv: bool):  # noqa: ANN001, ANN202
+        """q/k norm + RoPE of layer ``li`` and its K/V rows into the cache; k and v are None where an 8-bit decode needs neither."""
+        if self.kv_fp8 is not None:
+            return paged_fp8.qk_norm_rope_cache_fp8(qkv, a.q_norm, a.k_norm, pos, inv, a.nq, a.nkv, a.eps, self._kv8(li), slots, want_kv=want_kv)
+        return paged.qk_norm_rope_cache(qkv, a.q_norm, a.k_norm, pos, inv, a.nq, a.nkv, a.eps, self.kv[li, 0], self.kv[li, 1], slots)
+
+    def _kv8(self, li: int) -> paged_fp8.Fp8KV:
+        return paged_fp8.layer_cache(self.kv_fp8[0][li], self.kv_fp8[1][li])
+
+    def _copy_page(self, dst: int, src: int) -> None:
+        for t in (self.kv,) if self.kv_fp8 is None else (x.view(torch.uint8) for x in self.kv_fp8):
+            t[:, :, dst].copy_(t[:, :, src])
+
+    def _layers_tp(self, h, pos, slots, attend, want_kv=True):  # noqa: ANN001, ANN202
         """TP forward: local-shard GEMMs, one fused all-reduce + residual + RMSNorm after each
         row-parallel projection.  Returns the final normed hidden state."""
         tp, e, eps = self.tp, _ext.ext(), self.cfg.rms_norm_eps
@@ -299,7 +337,7 @@ class RolloutEngine:
         for li, layer in enumerate(layers):
             a = layer.self_attn
             qkv = self._lin(x, a.qkv_proj)
-            q, k, v = paged.qk_norm_rope_cache(qkv, a.q_norm, a.k_norm, pos, inv, a.nq, a.nkv, a.eps, self.kv[li, 0], self.kv[li, 1], slots)
+            q, k, v = self._append_kv(li, a, qkv, pos, inv, slots, want_kv)
             o = a.gate_output(attend(li, q, k, v).reshape(rows, -1), x, self._lin)
             self._lin_into(o, a.o_proj, tp.partial_buffer(rows))
             h, x = tp.allreduce_rms(rows, h, layer.post_attention_layernorm.weight, eps)
@@ -326,10 +364,10 @@ class RolloutEngine:
         return (self.is_cuda and not self.fp8 and 1 <= rows <= 128 and self.cfg.hidden_size % 64 == 0
                 and os.environ.get("AXRL_DECODE_FOLD", "0") == "1")
 
-    def _layers(self, h, pos, slots, attend, capture=None, mix=None):  # noqa: ANN001, ANN202
+    def _layers(self, h, pos, slots, attend, capture=None, mix=None, want_kv=True):  # noqa: ANN001, ANN202
         """``mix(li, module, x)``: the token mixer of linear-attention layers (hybrid models)."""
         if self.tp is not None:
-            return self._layers_tp(h, pos, slots, attend)
+            return self._layers_tp(h, pos, slots, attend, want_kv)
         inv = self.model.inv_freq
         fold = self._fold_elementwise(h.shape[0])
         e = _ext.ext() if fold else None
@@ -348,8 +386,7 @@ class RolloutEngine:
             else:
                 x = self._rms(h, layer.input_layernorm.weight)
                 qkv = self._lin(x, a.qkv_proj)
-            q, k, v = paged.qk_norm_rope_cache(qkv, a.q_norm, a.k_norm, pos, inv, a.nq, a.nkv, a.eps,
-                                               self.kv[li, 0], self.kv[li, 1], slots)
+            q, k, v = self._append_kv(li, a, qkv, pos, inv, slots, want_kv)
             o = a.gate_output(attend(li, q, k, v).reshape(q.shape[0], -1), x, self._lin)
             h = self._lin(o, a.o_proj, residual=h)
             if fold and not hasattr(layer.mlp, "router"):
@@ -504,31 +541,55 @@ class RolloutEngine:
     def _prefill(self, groups: list[list[GenRequest]]) -> list[GenResult]:
         t0 = time.perf_counter()
         ids, pos, slots, triples, lasts = [], [], [], [], []
+        prefix_slots: list[int] = []  # cached rows that the new ones attend to: the first keys, the new rows' follow
+        prefix_triples = []
         protos: list[_Seq] = []
         off = 0
+        capture = {} if self.cfg.is_moe and any(m.capture_routing for g in groups for m in g) else None
+        # captured routing needs every prompt row; linear-attention layers need their states
+        reuse = self.kv_fp8 is not None and capture is None and not self.gdn_index
         for members in groups:
             r0 = members[0]
             n = len(r0.prompt)
             assert 0 < n < self.max_context, f"prompt length {n} out of range"
-            pages = self.bm.allocate(self._pages_needed(n))
-            protos.append(_Seq(r0, list(r0.prompt), pages))
-            ids.extend(r0.prompt)
-            pos.extend(range(n))
+            shared, c0 = self.bm.match_prefix(list(r0.prompt)) if reuse else ([], 0)
+            if c0 == n:  # the last token is computed: its logits are needed
+                self.bm.release([shared.pop()])
+                c0 -= self.P
+            pages = list(shared) + self.bm.allocate(self._pages_needed(n) - len(shared))
+            protos.append(_Seq(r0, list(r0.prompt), pages, cached=c0))
+            ids.extend(r0.prompt[c0:])
+            pos.extend(range(c0, n))
             pg = np.asarray(pages, dtype=np.int64)
             ar = np.arange(n)
-            slots.extend((pg[ar // self.P] * self.P + ar % self.P).tolist())
-            triples.append((off, off + n, off, off + n, 1))
-            lasts.append(off + n - 1)
-            off += n
+            sl = (pg[ar // self.P] * self.P + ar % self.P).tolist()
+            slots.extend(sl[c0:])
+            m = n - c0
+            triples.append((off, off + m, off, off + m, 1))
+            if c0:
+                prefix_triples.append((off, off + m, len(prefix_slots), len(prefix_slots) + c0, 0))
+                prefix_slots.extend(sl[:c0])
+            lasts.append(off + m - 1)
+            off += m
         dev = self.device
         ids_t = torch.tensor(ids, dtype=torch.int64).to(dev, non_blocking=True)
         pos_t = torch.tensor(pos, dtype=torch.int32).to(dev, non_blocking=True)
         slots_t = torch.tensor(slots, dtype=torch.int64).to(dev, non_blocking=True)
-        spec = spec_from_triples(triples, off)
+        Tp = len(prefix_slots)
+        prefix_t = torch.tensor(prefix_slots, dtype=torch.int64).to(dev, non_blocking=True)
+        spec = spec_from_triples(prefix_triples + [(q0, q1, Tp + k0, Tp + k1, t) for q0, q1, k0, k1, t in triples], off, Tp + off)
         if self.is_cuda:
             spec = spec.to(dev)
-            iostats.add_h2d(ids_t, pos_t, slots_t, spec.qseg, spec.kr, spec.kseg, spec.qr, spec.fwd_tiles, spec.bwd_tiles)
-        capture = {} if self.cfg.is_moe and any(m.capture_routing for g in groups for m in g) else None
+            iostats.add_h2d(ids_t, pos_t, slots_t, prefix_t, spec.qseg, spec.kr, spec.kseg, spec.qr, spec.fwd_tiles, spec.bwd_tiles)
+
+        def attend(li: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+            if Tp:
+                kv = torch.empty(2, Tp + off, *k.shape[1:], dtype=torch.bfloat16, device=dev)
+                paged_fp8.gather_kv_fp8(self._kv8(li), prefix_t, kv[0, :Tp], kv[1, :Tp])
+                kv[0, Tp:], kv[1, Tp:] = k, v
+                k, v = kv.to(k.dtype)
+            return ops.attention(q, k, v, spec)
+
         lslots = [[self.gdn_free.pop() for _ in members] for members in groups] if self.gdn_index else None
 
         def gdn_prefill(li: int, a, x: torch.Tensor) -> torch.Tensor:  # noqa: ANN001
@@ -543,7 +604,7 @@ class RolloutEngine:
 
         with torch.no_grad():
             h = self._embed(ids_t)
-            h = self._layers(h, pos_t, slots_t, lambda li, q, k, v: ops.attention(q, k, v, spec), capture, mix=gdn_prefill)
+            h = self._layers(h, pos_t, slots_t, attend, capture, mix=gdn_prefill)
             logits = self._logits(h.index_select(0, torch.tensor(lasts, device=dev)))
         rows, temps, rids, forced = [], [], [], []
         new_seqs: list[_Seq] = []
@@ -560,8 +621,8 @@ class RolloutEngine:
                     self.bm.incref(shared)
                     extra = self.bm.allocate(len(proto.pages) - full)
                     if extra:
-                        self.kv[:, :, extra[0]].copy_(self.kv[:, :, proto.pages[full]])
-                    s = _Seq(r, list(r.prompt), shared + extra)
+                        self._copy_page(extra[0], proto.pages[full])
+                    s = _Seq(r, list(r.prompt), shared + extra, cached=proto.cached)
                 s.stream = r.seed_stream if r.seed_stream is not None else _stream_id(r.rid)
                 if lslots is not None:
                     s.lslot = lslots[gi][mi]
@@ -900,8 +961,12 @@ class RolloutEngine:
             self.gdn_S[gi].index_copy_(0, lsl, S)
             return out
 
-        h = self._layers(h, pos, slots, lambda li, q, k, v: paged.paged_decode_attention(q, self.kv[li, 0], self.kv[li, 1], bt, lens, self.ws, planned=True),
-                         capture, mix=gdn_decode)
+        def attend(li: int, q: torch.Tensor, k, v) -> torch.Tensor:  # noqa: ANN001
+            if self.kv_fp8 is not None:
+                return paged_fp8.paged_decode_attention_fp8(q, self._kv8(li), bt, lens)
+            return paged.paged_decode_attention(q, self.kv[li, 0], self.kv[li, 1], bt, lens, self.ws, planned=True)
+
+        h = self._layers(h, pos, slots, attend, capture, mix=gdn_decode, want_kv=False)
         logits = self._logits(h)
         if self.filtered_mode:
             t, l = paged.sample_filtered(logits, st["temp"][:bucket], st["top_k"][:bucket], st["top_p"][:bucket], st["min_p"][:bucket],
@@ -960,6 +1025,8 @@ class RolloutEngine:
             p1.copy_(p2, non_blocking=True)
         if self.weight_format == "fp8_block":
             self.quantize_weights()
+        if self.kv_fp8 is not None:  # prompts attend to cached pages: none of the old weights' may remain
+            self.reset_prefix_cache()
 
     def reset_prefix_cache(self) -> None:
         """Weights changed: cached pages no longer match (the reference flushes its radix cache)."""
