@@ -511,27 +511,27 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   int nj = 0, row = -1;     // next tile to load (even: K, odd: V of the same unit), its cache row
   bool new_pair = true;     // of `ld`: its q rows come with its K tile
   auto load_next = [&] {
-    if ((nj & 1) == 0) {
+    const bool is_k = (nj & 1) == 0;
+    if (is_k) {
       if (ld.left <= 0) return;
-      if (new_pair && lane == 0) {
-        const int bytes = p.G * D * 2;
-        tc::mbar_tx(&full[nj % SLOTS], bytes);  // counted before the arrival below completes the phase
-        bulk_bytes(sq, p.q + ((long)ld.b * p.Hkv + ld.hk) * p.G * D, bytes, &full[nj % SLOTS]);
-      }
       row = ld.page >= 0 ? (int)(((long)ld.page * p.Hkv + ld.hk) * p.P) + ld.off : -1;
-      next_unit(ld);
-      if (ld.left > 0) {
-        new_pair = ld.u == 0;
-        fetch_page(ld);
-      }
     }
     const int s = nj % SLOTS;
     if (loads) {
       reinterpret_cast<uint8_t*>(&meta[s])[lane] = row >= 0;
-      tc::mbar_expect_tx(&full[s], row >= 0 ? p.box * (D + 1) : 0);
+      const int q_bytes = is_k && new_pair && lane == 0 ? p.G * D * 2 : 0;
+      tc::mbar_expect_tx(&full[s], (row >= 0 ? p.box * (D + 1) : 0) + q_bytes);
       if (row >= 0) {
-        tc::tma_2d(ring + s * TILE + lane * p.box * D, (nj & 1) ? &tv : &tk, 0, row, &full[s]);
-        bulk_bytes(sc + s * UNIT + lane * p.box, ((nj & 1) ? p.vs : p.ks) + row, p.box, &full[s]);
+        tc::tma_2d(ring + s * TILE + lane * p.box * D, is_k ? &tk : &tv, 0, row, &full[s]);
+        bulk_bytes(sc + s * UNIT + lane * p.box, (is_k ? p.ks : p.vs) + row, p.box, &full[s]);
+      }
+      if (q_bytes) bulk_bytes(sq, p.q + ((long)ld.b * p.Hkv + ld.hk) * p.G * D, q_bytes, &full[s]);
+    }
+    if (is_k) {
+      next_unit(ld);
+      if (ld.left > 0) {
+        new_pair = ld.u == 0;
+        fetch_page(ld);
       }
     }
     ++nj;
@@ -597,19 +597,23 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
 #pragma unroll
       for (int t = 0; t < NT; ++t) s[t][i16][0] = s[t][i16][1] = s[t][i16][2] = s[t][i16][3] = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 4; ++k) {
+      uint32_t x[4][8];
 #pragma unroll
-      for (int i16 = 0; i16 < 4; ++i16) {  // innermost: the four tiles' sums do not depend on each other
-        uint32_t a[4], x[8];
+      for (int i16 = 0; i16 < 4; ++i16) {
+        uint32_t a[4];
         ldsm4(a, ring_a + sk * TILE + i16 * 16 * D + k_off[k]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) halves(a[e], x[2 * e], x[2 * e + 1]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          mma_f16(s[t][i16], x[0], x[2], x[1], x[3], qf[t][4 * k], qf[t][4 * k + 1]);
-          mma_f16(s[t][i16], x[4], x[6], x[5], x[7], qf[t][4 * k + 2], qf[t][4 * k + 3]);
-        }
+        for (int e = 0; e < 4; ++e) halves(a[e], x[i16][2 * e], x[i16][2 * e + 1]);
       }
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i16 = 0; i16 < 4; ++i16)  // innermost: the four tiles' sums do not depend on each other
+            mma_f16(s[t][i16], x[i16][4 * half], x[i16][4 * half + 2], x[i16][4 * half + 1], x[i16][4 * half + 3], qf[t][4 * k + 2 * half], qf[t][4 * k + 2 * half + 1]);
+    }
 #pragma unroll
     for (int i16 = 0; i16 < 4; ++i16) {
       const float ka = scale_value(sc[sk * UNIT + i16 * 16 + tok_a]), kb = scale_value(sc[sk * UNIT + i16 * 16 + tok_b]);
