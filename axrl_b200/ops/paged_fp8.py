@@ -99,8 +99,8 @@ def qk_norm_rope_cache_fp8(qkv: torch.Tensor, qw: torch.Tensor, kw: torch.Tensor
 
     Returns q and, with ``want_kv``, k and v as the cache stands for them (bf16, exact): a prefill that attends to
     these sees what later decode steps and :func:`gather_kv_fp8` see.  Without it both are None (decode)."""
-    check_full_rotary(qw, inv_freq)
     if not qkv.is_cuda:
+        check_full_rotary(qw, inv_freq)
         T, dim = qkv.shape[0], qw.numel()
         q, k, v = qkv.view(T, nq + 2 * nkv, dim).float().split([nq, nkv, nkv], 1)
         q = _rope64(_rms_ref(q, qw, eps), pos, inv_freq).to(qkv.dtype)

@@ -353,14 +353,15 @@ def test_append_decode_load_together(dev):
 
 
 @pytest.mark.gpu
-def test_captured_steps_replay_on_a_side_stream():
+@pytest.mark.parametrize("lens", [[100, 1, 64, 65, 300, 20], [5000, 0, 900, 1, 2000, 777]])
+def test_captured_steps_replay_on_a_side_stream(lens):
     """Append + decode captured into two graphs that are replayed in turn on another stream, with new inputs in place."""
     nq, nkv, P, B = 8, 2, 64, 6
-    lens = [100, 1, 64, 65, 300, 20]
     q0, cache, bt, L = _decode_case(lens, nq, nkv, P, "cuda")
     qkv, qw, kw, pos, inv = _inputs(B, nq, nkv, "cuda")
     pos.copy_(L - 1)
-    slots = bt.long().gather(1, ((L - 1) // P).long()[:, None])[:, 0] * P + (L - 1).long() % P
+    slots = bt.long().gather(1, ((L - 1).clamp_min(0) // P).long()[:, None])[:, 0] * P + (L - 1).long() % P
+    slots = torch.where(L > 0, slots, torch.full_like(slots, -1))
 
     def step():
         q, _, _ = pf.qk_norm_rope_cache_fp8(qkv, qw, kw, pos, inv, nq, nkv, EPS, cache, slots, want_kv=False)
