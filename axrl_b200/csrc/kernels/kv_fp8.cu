@@ -77,7 +77,9 @@ __global__ void __launch_bounds__(AW * 32, 4) append_k(const bf16* __restrict__ 
                                                        const int* __restrict__ pos, const float* __restrict__ inv_freq, bf16* __restrict__ q,
                                                        bf16* __restrict__ ko, bf16* __restrict__ vo, int T, int nq, int nkv, float eps, Cache c,
                                                        const int64_t* __restrict__ slots, int parts) {
-  // [token][q, k][i][l]: wa cos, wb sin, wb cos, wa sin of pair 8 l + i; eight lanes read 128 consecutive bytes
+  // [token][q, k][i][l] for pair 8 l + i; eight lanes read 128 consecutive bytes.  q: wa cos, wb sin, wb cos, wa sin.
+  // k: wa, wb, cos, sin: a key is rounded to e4m3, whose borders turn a difference in the last bit into a whole code, so
+  // keys are computed in the order of the definition, each factor rounded once.
   __shared__ float4 s_w[AW / 2][2][8][8];
   pdl_trigger();
   pdl_wait();
@@ -103,14 +105,11 @@ __global__ void __launch_bounds__(AW * 32, 4) append_k(const bf16* __restrict__ 
     if (t0 + ti < T) {
       double a = (double)pos[t0 + ti] * 0.15915494309189535 * (double)inv_freq[f];  // in turns: 1 / (2 pi)
       a -= rint(a);
-      float sn, cs;
-      sincospif((float)(2.0 * a), &sn, &cs);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const bf16* w = k ? kw : qw;
-        const float wa = __bfloat162float(w[f]), wb = __bfloat162float(w[f + 64]);
-        s_w[ti][k][f & 7][f >> 3] = make_float4(wa * cs, wb * sn, wb * cs, wa * sn);
-      }
+      double sd, cd;
+      sincospi(2.0 * a, &sd, &cd);
+      const float sn = (float)sd, cs = (float)cd, wa = __bfloat162float(qw[f]), wb = __bfloat162float(qw[f + 64]);
+      s_w[ti][0][f & 7][f >> 3] = make_float4(wa * cs, wb * sn, wb * cs, wa * sn);
+      s_w[ti][1][f & 7][f >> 3] = make_float4(__bfloat162float(kw[f]), __bfloat162float(kw[f + 64]), cs, sn);
     }
   }
   const bool live = slot >= 0 && slot < c.pages * c.P;
@@ -135,9 +134,15 @@ __global__ void __launch_bounds__(AW * 32, 4) append_k(const bf16* __restrict__ 
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float4 w = s_w[tt][isq ? 0 : 1][i][l8];
-        const float x = a[i] * r, y = b[i] * r;
-        a[i] = x * w.x - y * w.y;
-        b[i] = y * w.z + x * w.w;
+        float x = a[i] * r, y = b[i] * r;
+        if (isq) {
+          a[i] = x * w.x - y * w.y;
+          b[i] = y * w.z + x * w.w;
+        } else {
+          x *= w.x, y *= w.y;
+          a[i] = __fsub_rn(__fmul_rn(x, w.z), __fmul_rn(y, w.w));
+          b[i] = __fadd_rn(__fmul_rn(y, w.z), __fmul_rn(x, w.w));
+        }
       }
     }
     if (isq) {

@@ -41,13 +41,15 @@ def _same(a, b, atol):
     """Greedy runs of the same computation.  Where logits differ by at most d, the largest one differs by at most d too, so the
     log-probs agree up to and at the first token that differs, and from there on the texts are not the same any more."""
     n = next((i for i, (x, y) in enumerate(zip(a.output_ids, b.output_ids)) if x != y), len(a.output_ids) - 1) + 1
-    assert len(a.output_ids) == len(b.output_ids) and (atol > 1e-3 or n == len(a.output_ids))
+    assert len(a.output_ids) == len(b.output_ids)
     torch.testing.assert_close(torch.tensor(a.output_logprobs[:n]), torch.tensor(b.output_logprobs[:n]), atol=atol, rtol=0)
 
 
-# fp32 on the CPU.  On the GPU the products' order, and so the rounding, depends on the number of rows: logits of this model
+# A product's rounding depends on the number of rows it is computed with, in the last bit on the CPU (fp32); a key next to the
+# border between two codes then moves by a code, 2^-3 of it, and a score by 2^-3 |q_i k_i| / sqrt(128) < 0.02 of products below
+# 2: fewer than one in 10^5 do.  On the GPU the products' order, and so the rounding, depends on the number of rows: logits of this model
 # stay below 4 in size and are rounded to bf16, 2^-8 x 4 in each of two runs, and as much again from the hidden states.
-ATOL = {"cpu": 1e-4, "cuda": 4 * 2.0 ** -8 * 4}
+ATOL = {"cpu": 0.02, "cuda": 4 * 2.0 ** -8 * 4}
 
 
 @pytest.mark.parametrize("dev", ["cpu", CUDA])
