@@ -19,14 +19,15 @@ namespace kv8 {
 
 constexpr int D = 128;
 
-// The least power of two s with amax <= 448 s, as its e8m0 byte: amax = 1.m x 2^x, 448 = 1.75 x 2^8.
+// The least power of two s >= 2^-60 with amax <= 448 s, as its e8m0 byte: amax = 1.m x 2^x, 448 = 1.75 x 2^8.  The bound (values
+// below 4e-16 lose bits, at most 2^-70 of error) keeps the scales of a sequence within what the decode's weights span.
 // `bits`: the largest |value| as raw bits (an unsigned maximum of these keeps infinities and NaN).
 __device__ __forceinline__ uint32_t scale_byte(uint32_t bits) {
   const uint32_t x = bits >> 23;
   if (x == 255u) return 255u;  // not finite: the row stands for NaN
   if (bits == 0u) return 127u;
   const int e = (int)x - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return (uint32_t)max(e, 1);
+  return (uint32_t)max(e, 127 - 60);
 }
 __device__ __forceinline__ float scale_value(uint32_t byte) { return byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte ? byte << 23 : 0x400000u); }
 // 1 / scale, 0 for a row that is not finite (its codes are 0).
@@ -63,7 +64,8 @@ struct Cache {
 // token: a' = r (a wa cos - b wb sin), b' = r (b wb cos + a wa sin).  A warp works on four heads at a time, a quarter-warp
 // each: lane l of 8 holds elements 8l .. 8l + 7 of both halves, so a rotation pair stays in one thread and every access is 16
 // bytes (codes: 8); the next four heads are loaded before the current ones are computed.  16384 tokens of 32 q and 8 kv
-// heads: one warp walking a token with its own angles 100 us, products in registers 113 us (14 warps an SM), this form TODO.
+// heads: one warp walking a token with its own angles 100 us, products in registers 113 us (14 warps an SM), this form 79 us,
+// 84 % of the measured copy rate; 2049 tokens of 16 q and 8 kv heads 9.3 us (floor 5.8).
 constexpr int AW = 8;  // warps
 
 // Largest magnitude, a NaN if there is one (the sign of the result means nothing).
@@ -80,34 +82,36 @@ __global__ void __launch_bounds__(AW * 32, 4) append_k(const bf16* __restrict__ 
   // [token][q, k][i][l] for pair 8 l + i; eight lanes read 128 consecutive bytes.  q: wa cos, wb sin, wb cos, wa sin.
   // k: wa, wb, cos, sin: a key is rounded to e4m3, whose borders turn a difference in the last bit into a whole code, so
   // keys are computed in the order of the definition, each factor rounded once.
-  __shared__ float4 s_w[AW / 2][2][8][8];
+  __shared__ float4 s_w[AW][2][8][8];
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7, tokens = AW / parts;
   const int t0 = blockIdx.x * tokens;
   const int tt = warp / parts, part = warp % parts, t = t0 + tt;
-  const int gq = (nq + 3) >> 2, gk = (nkv + 3) >> 2, groups = gq + 2 * gk;  // of four heads: q, then k, then v
+  const int gq = (nq + 3) >> 2, groups = gq + ((2 * nkv + 3) >> 2);  // of four heads: q, then k and v
   const int g0 = groups * part / parts, g1 = groups * (part + 1) / parts;
   const bool any = t < T && g0 < g1;
   const bf16* src = qkv + (long)t * (nq + 2 * nkv) * D + 8 * l8;
   uint4 na = make_uint4(0, 0, 0, 0), nb = na;
   auto fetch = [&](int g) {
-    const int skip = g < gq ? 0 : g < gq + gk ? gq : gq + gk, h = 4 * (g - skip) + (lane >> 3);
-    if (h < (g < gq ? nq : nkv)) {
-      const bf16* at = src + (h + (g < gq ? 0 : g < gq + gk ? nq : nq + nkv)) * D;
+    const int h = 4 * (g < gq ? g : g - gq) + (lane >> 3);
+    if (h < (g < gq ? nq : 2 * nkv)) {
+      const bf16* at = src + (h + (g < gq ? 0 : nq)) * D;
       na = *reinterpret_cast<const uint4*>(at), nb = *reinterpret_cast<const uint4*>(at + 64);
     }
   };
   if (any) fetch(g0);
   const long slot = any ? slots[t] : -1;
-  if ((int)threadIdx.x < tokens * (D / 2)) {
-    const int ti = threadIdx.x / (D / 2), f = threadIdx.x % (D / 2);
+  for (int i = threadIdx.x; i < tokens * (D / 2); i += AW * 32) {
+    const int ti = i / (D / 2), f = i % (D / 2);
     if (t0 + ti < T) {
-      double a = (double)pos[t0 + ti] * 0.15915494309189535 * (double)inv_freq[f];  // in turns: 1 / (2 pi)
-      a -= rint(a);
-      double sd, cd;
-      sincospi(2.0 * a, &sd, &cd);
-      const float sn = (float)sd, cs = (float)cd, wa = __bfloat162float(qw[f]), wb = __bfloat162float(qw[f + 64]);
+      double turns = (double)pos[t0 + ti] * 0.15915494309189535 * (double)inv_freq[f];  // 1 / (2 pi)
+      turns = 2.0 * (turns - rint(turns));
+      const float x = (float)turns, rest = (float)(turns - (double)x) * 3.14159265f;
+      float s0, c0;
+      sincospif(x, &s0, &c0);
+      const float sn = fmaf(c0, rest, s0), cs = fmaf(-s0, rest, c0);  // what the rounding of x left out
+      const float wa = __bfloat162float(qw[f]), wb = __bfloat162float(qw[f + 64]);
       s_w[ti][0][f & 7][f >> 3] = make_float4(wa * cs, wb * sn, wb * cs, wa * sn);
       s_w[ti][1][f & 7][f >> 3] = make_float4(__bfloat162float(kw[f]), __bfloat162float(kw[f + 64]), cs, sn);
     }
@@ -117,14 +121,15 @@ __global__ void __launch_bounds__(AW * 32, 4) append_k(const bf16* __restrict__ 
   __syncthreads();
   if (!any) return;
   for (int g = g0; g < g1; ++g) {
-    const bool isq = g < gq, isv = g >= gq + gk;
-    const int h = 4 * (g - (isq ? 0 : isv ? gq + gk : gq)) + (lane >> 3);
-    const bool in = h < (isq ? nq : nkv);
+    const bool isq = g < gq;
+    int h = 4 * (isq ? g : g - gq) + (lane >> 3);
+    const bool in = h < (isq ? nq : 2 * nkv), isv = !isq && h >= nkv;
+    if (isv) h -= nkv;
     float a[8], b[8];
     load8(reinterpret_cast<const bf16*>(&na), a);
     load8(reinterpret_cast<const bf16*>(&nb), b);
     if (g + 1 < g1) fetch(g + 1);
-    if (!isv) {
+    if (!__all_sync(0xffffffffu, isv)) {
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
@@ -140,8 +145,8 @@ __global__ void __launch_bounds__(AW * 32, 4) append_k(const bf16* __restrict__ 
           b[i] = y * w.z + x * w.w;
         } else {
           x *= w.x, y *= w.y;
-          a[i] = __fsub_rn(__fmul_rn(x, w.z), __fmul_rn(y, w.w));
-          b[i] = __fadd_rn(__fmul_rn(y, w.z), __fmul_rn(x, w.w));
+          const float ra = __fsub_rn(__fmul_rn(x, w.z), __fmul_rn(y, w.w)), rb = __fadd_rn(__fmul_rn(y, w.z), __fmul_rn(x, w.w));
+          a[i] = isv ? a[i] : ra, b[i] = isv ? b[i] : rb;  // a group may hold keys and values
         }
       }
     }
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(AW * 32, 4) append_k(const bf16* __restrict__ 
 // Rows of the cache as bf16 (exact): 129 bytes in and 256 out for each of the 2 Hkv rows of a slot, bound by that.  A warp
 // takes 16 rows (the rows of one slot with eight heads): lane i looks up row i, then two rows at a time are converted, 16
 // lanes of 8 codes each, so that a store fills 512 bytes; all 16 rows are read before the first is written.  One thread per
-// 16 codes, each looking up its own slot, took 395 us for 131072 slots (floor 123), this form TODO.
+// 16 codes, each looking up its own slot, took 395 us for 131072 slots of eight heads, this form 132 us, 94 % of the measured copy rate.
 constexpr int LR = 16;
 
 __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict__ slots, bf16* __restrict__ ko, bf16* __restrict__ vo, long rows) {
@@ -255,11 +260,12 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // group fill the n = 8 columns; groups of 9 to 16 take two column tiles.  The e4m3 form of mma.sync needs no conversions in
 // the source but is no faster here: measured 5.4 clk per 16 x 32 step on an SM with two 8-bit terms per head, against 6.3
 // clk for the load, conversions and two products above, which serve twice the heads (256 short sequences with groups of
-// eight: 56.5 us against TODO).
+// eight: 56.5 us against 40.4).
 //
 // Softmax in the log2 domain on w_t = scale log2(e) q.k_t + e_t, the exponent of V folded in: P_t = 2^{w_t - max w} <= 1
 // rounds to f16 (2^-11, finer than bf16) and multiplies the codes themselves, and the normaliser is l = sum P_t 2^{-e_t}
-// in fp32, unrounded.  Whatever falls below f16 is 2^-24 of the largest weighted term.  q rows are scaled by a power of
+// in fp32, unrounded.  Whatever falls below f16 is 2^-24 of the largest weighted term; P itself leaves fp32 (and l) only where
+// exponents of V in a sequence lie 100 and more apart, which scales of at least 2^-60 do not below |v| = 10^14.  q rows are scaled by a power of
 // two so that their largest is in [2^14, 2^15) and round to f16 exactly but for what is below 2^-28 of it.
 constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 2, TILE = UNIT * D;  // TILE: bytes of one slot
 constexpr int MAXB = 2048, DIRECT_TOKENS = NW * UNIT;
@@ -822,7 +828,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
 // those CTAs; zeros for empty sequences.  CTA i looks for the pair that goes on behind CTA i before decode_k has ended; then
 // its MW warps are dealt to the heads of the group and, where those are fewer, to stripes of the partials, whose loads
 // are all in flight at once.  One warp walking the partials of all warps took 42 us for two contexts of 100k, CTAs of
-// eight warps for every pair 6 us, and 5 us for 256 short sequences; this form TODO.
+// eight warps for every pair 6 us, and 5 us for 256 short sequences; this form 2 us.
 constexpr int MW = 8, MBATCH = 4;
 
 __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
@@ -942,10 +948,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qknorm_rope_cache_fp8(const at::T
   at::Tensor ko, vo;
   if (want_kv) ko = at::empty({T, nkv, D}, opt), vo = at::empty({T, nkv, D}, opt);
   if (T == 0) return {q, ko, vo};
-  // Warps per token: eight until the SMs have some sixteen CTAs each (a single token: 2.9 us either way), then fewer, which
-  // share the products of weights and angles among more heads (16384 tokens: TODO).
-  const int64_t many = (int64_t)num_sms() * 4;
-  const int parts = T <= many ? 8 : T <= 2 * many ? 4 : 2;
+  // Warps per token.  Few tokens: eight, for latency (64 tokens of 32 q and 8 kv heads 2.9 us, 5.1 with two).  Many: two, as
+  // many tokens as a CTA then has share its start (16384 tokens 79 us, 85 with four and 107 with eight; 1024 tokens 7.4 us
+  // with eight, 6.8 with four, 11.0 with two), or one where a token has few heads (8 q and 1 kv head, 16384 tokens: 29 us,
+  // 32 with two; 2049 tokens: 8.1 us, 5.3 with two).
+  const int64_t many = (int64_t)num_sms() * 4, groups = (nq + 3) / 4 + (2 * nkv + 3) / 4;
+  const int parts = T <= many ? 8 : T <= 2 * many ? 4 : groups < 8 && T > 8 * many ? 1 : 2;
   launch_pdl(append_k, dim3((unsigned)((T + AW / parts - 1) / (AW / parts))), dim3(AW * 32), 0, stream(), (const bf16*)qkv.data_ptr(), (const bf16*)qw.data_ptr(),
              (const bf16*)kw.data_ptr(), (const int*)pos.data_ptr(), (const float*)inv_freq.data_ptr(), (bf16*)q.data_ptr(),
              (bf16*)(want_kv ? ko.data_ptr() : nullptr), (bf16*)(want_kv ? vo.data_ptr() : nullptr), (int)T, (int)nq, (int)nkv, (float)eps, c,

@@ -43,13 +43,13 @@ def layer_cache(codes: torch.Tensor, scales: torch.Tensor) -> Fp8KV:
 
 
 def quantize_rows_e8m0(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """Rows ``(..., D)`` to e4m3 codes and their e8m0 scales ``(...)``: the least power of two with
+    """Rows ``(..., D)`` to e4m3 codes and their e8m0 scales ``(...)``: the least power of two, 2^-60 or more, with
     ``amax <= 448 * scale`` (1 for a row of zeros, NaN with codes 0 for a row that is not finite)."""
     xf = x.float()
     amax = xf.abs().amax(-1)
     ok = amax.isfinite() & xf.isfinite().all(-1)
     m, e = torch.frexp(torch.where(ok, amax, torch.ones_like(amax)))
-    e = (e - 9 + (m > 0.875).to(e.dtype)).clamp_min(-126)
+    e = (e - 9 + (m > 0.875).to(e.dtype)).clamp_min(-60)
     e = torch.where(amax == 0, torch.zeros_like(e), e)
     codes = torch.where(ok[..., None], torch.ldexp(xf, -e[..., None]), torch.zeros_like(xf)).to(torch.float8_e4m3fn)
     byte = torch.where(ok, e + 127, torch.full_like(e, 255)).to(torch.uint8)

@@ -61,7 +61,7 @@ def _at(t, slots):
 # ----------------------------------------------------------------------------- quantisation
 def test_quantize_rows_scale_is_the_least_power_of_two():
     g = torch.Generator().manual_seed(1)
-    x = torch.randn(4000, D, generator=g) * torch.exp2(torch.randint(-60, 60, (4000, 1), generator=g).float())
+    x = torch.randn(4000, D, generator=g) * torch.exp2(torch.randint(-45, 60, (4000, 1), generator=g).float())
     x[0] = 0
     x[1, 0], x[1, 1:] = 448.0, 1.0  # on the border: scale 1
     x[2, 0], x[2, 1:] = 448.5, 1.0  # past it: scale 2
@@ -150,6 +150,23 @@ def test_append_skips_slots_outside_the_cache_and_takes_no_tokens(dev):
         assert torch.equal(now[keep], was[keep])
     q, k, v = pf.qk_norm_rope_cache_fp8(qkv[:0], qw, kw, pos[:0], inv, 4, 2, EPS, cache, slots[:0])
     assert q.shape == (0, 4, D) and k.shape == (0, 2, D) and v.shape == (0, 2, D)
+
+
+@pytest.mark.parametrize("dev", ["cpu", CUDA])
+def test_append_tiny_values(dev):
+    """No scale is below 2^-60; a row next to ones of ordinary size still takes its share of the weights when it is nearly zero."""
+    cache = _cache(1, 1, 16, dev)
+    qkv, qw, kw, pos, inv = _inputs(6, 1, 1, dev)
+    x = qkv.view(6, 3, D)
+    x[1, 2] *= 2.0 ** -55
+    x[2, 2] *= 2.0 ** -120
+    x[3, 2, 1:] = 0
+    x[3, 2, 0] = 2.0 ** -133  # the smallest bf16
+    q, _, v = pf.qk_norm_rope_cache_fp8(qkv, qw, kw, pos, inv, 1, 1, EPS, cache, torch.arange(6, device=dev))
+    assert cache.v_scale.view(torch.uint8)[0, 0, :6].min() == 127 - 60
+    err = (v.double() - x[:, 2:].double()).abs()
+    assert (err <= torch.maximum(2.0 ** -4 * x[:, 2:].double().abs(), torch.full_like(err, 2.0 ** -70))).all()
+    _check_decode(q[:1], cache, torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.tensor([6], dtype=torch.int32, device=dev))
 
 
 @pytest.mark.parametrize("dev", ["cpu", CUDA])
