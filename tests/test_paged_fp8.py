@@ -120,16 +120,16 @@ def _check_append(dev, T, nq, nkv, P, far, seed=0, want_kv=True):
 
 @pytest.mark.parametrize("dev", ["cpu", CUDA])
 @pytest.mark.parametrize("T,nq,nkv,P,far", [(1, 32, 8, 64, 5), (5, 4, 2, 64, 40), (33, 16, 8, 16, 100_000), (257, 20, 4, 32, 4096), (70, 1, 1, 128, 70),
-                                            (19, 8, 1, 7, 300)])
+                                            (19, 8, 1, 7, 300), (9, 6, 3, 64, 50), (3, 0, 2, 16, 9)])
 @pytest.mark.parametrize("want_kv", [True, False])
 def test_append(dev, T, nq, nkv, P, far, want_kv):
     _check_append(dev, T, nq, nkv, P, far, want_kv=want_kv)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [2048, 5003])
-def test_append_many_tokens(T):
-    _check_append("cuda", T, 32, 8, 64, 20000)
+@pytest.mark.parametrize("T,nq,nkv", [(700, 16, 8), (2048, 32, 8), (5003, 32, 8), (5003, 8, 1)])
+def test_append_many_tokens(T, nq, nkv):
+    _check_append("cuda", T, nq, nkv, 64, 20000)
 
 
 @pytest.mark.parametrize("dev", ["cpu", CUDA])
@@ -402,6 +402,49 @@ def test_captured_steps_replay_on_a_side_stream(lens):
             for q, o in outs:
                 assert ((o.double() - want).abs() <= tol).all()
     torch.cuda.current_stream().wait_stream(s)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A cache of 4.9 GB of codes each for K and V; rows in its last pages."""
+    pages, nkv, P = 75000, 8, 64
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    codes = [torch.empty(pages, nkv, P, D, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.empty(pages, nkv, P, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu) for _ in range(2)]
+    cache = pf.Fp8KV(*codes, *scales)
+    T = 150
+    order = torch.tensor([pages - 1, 3, pages - 2], dtype=torch.int32, device="cuda")
+    t = torch.arange(T, device="cuda")
+    slots = order.long()[t // P] * P + t % P
+    qkv, qw, kw, _, inv = _inputs(T, 16, nkv, "cuda")
+    q, k, v = pf.qk_norm_rope_cache_fp8(qkv, qw, kw, t.to(torch.int32), inv, 16, nkv, EPS, cache, slots)
+    gk, gv = pf.gather_kv_fp8(cache, slots)
+    assert torch.equal(gk, k) and torch.equal(gv, v)
+    assert torch.equal(k.double(), _values(_at(cache.k, slots), _at(cache.k_scale, slots)))
+    _check_decode(q[-1:], cache, order[None], torch.tensor([T], dtype=torch.int32, device="cuda"))
+    wide = torch.zeros(1, 40, dtype=torch.int32, device="cuda")
+    wide[0, :3] = order
+    _check_decode(q[-1:], cache, wide, torch.tensor([T], dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls on two streams, each with its own inputs, in flight together."""
+    cases = [_decode_case([4000, 77, 900, 64], 8, 2, 64, "cuda", seed=1), _decode_case([300, 2500, 1, 8000, 40], 16, 1, 16, "cuda", seed=2)]
+    want = [_exact_decode(*c, D ** -0.5) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, (s, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                got[i].append(pf.paged_decode_attention_fp8(*c))
+    torch.cuda.synchronize()
+    for outs, (o, tol) in zip(got, want):
+        for x in outs:
+            assert torch.equal(x, outs[0])  # the same order of sums every time
+            assert ((x.double() - o).abs() <= tol).all()
 
 
 # ----------------------------------------------------------------------------- refusals
