@@ -288,7 +288,6 @@ struct DecParams {
   float* part_o;       // (CTAs, 2, G, 128): of the pair that began before the CTA's ranges, of the one that goes on behind them
   float2* part_ml;     // (CTAs, 2, G): max, sum
   float* part_w;       // (CTAs, NW, G, 128), groups above eight: kept for the warps' first pairs
-  int ranges;          // most ranges: warps of decode_k
   long pages;
   int B, G, Hkv, P, max_pages, box;  // box: token rows of one TMA load, gcd(P, 64)
   float scale_log2;
@@ -309,15 +308,19 @@ __device__ __forceinline__ bool wait_tile(uint64_t* bar, uint32_t phase) {
 // unit u starts at cell 1 + 2 u, and a range does the units that start in it.  All ranges have the same even length, so as few
 // as possible: with lengths that differ by a unit the longer ones end alone (two contexts of 100k, 20 and 21 units: 71.2 us,
 // all 21: 69.3 us).  Two cells or more: a range inside a pair has a unit.
+// The ranges are dealt to the CTAs evenly, neighbours together: `base` of them, one more for the first `extra` CTAs.
 struct Ranges {
-  int len, n;
-  __device__ Ranges(int cells, int most) : len(((cells + most - 1) / most + 1) & ~1) {
-    len = max(len, 2);
+  int len, n, base, extra;
+  __device__ Ranges(int cells, int ctas) {
+    const int most = ctas * NW;
+    len = max(((cells + most - 1) / most + 1) & ~1, 2);
     n = (cells + len - 1) / len;
+    base = n / ctas, extra = n - base * ctas;
   }
   __device__ int lo(int r) const { return r * len; }
   __device__ int of(int x) const { return x / len; }
-  __device__ int per_cta(int ctas) const { return max((n + ctas - 1) / ctas, 1); }  // few units still use every SM
+  __device__ int first(int cta) const { return cta * base + min(cta, extra); }
+  __device__ int cta_of(int r) const { return r < extra * (base + 1) ? r / (base + 1) : extra + (r - extra * (base + 1)) / base; }
 };
 __device__ __forceinline__ int cells(int units) { return units > 0 ? 2 * units + 1 : 0; }
 
@@ -491,10 +494,10 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
       for (int i = threadIdx.x; i < p.G * D / 8; i += NW * 32) reinterpret_cast<uint4*>(p.out + (long)blockIdx.x * p.G * D)[i] = make_uint4(0, 0, 0, 0);
   } else {
     cell_prefix<NW * 32>(p, prefix, s_len, s_warp);
-    const Ranges rg(prefix[p.B] * p.Hkv, gridDim.x * NW);
-    wpc = rg.per_cta(gridDim.x);
-    const int r = blockIdx.x * wpc + warp;
-    if (warp < wpc && r < rg.n) {
+    const Ranges rg(prefix[p.B] * p.Hkv, gridDim.x);
+    const int r = rg.first(blockIdx.x) + warp;
+    wpc = rg.first(blockIdx.x + 1) - rg.first(blockIdx.x);
+    if (warp < wpc) {
       const int x0 = rg.lo(r);
       b = sequence_of(prefix, p.B, x0 / p.Hkv, lane);
       const int pc = prefix[b + 1] - prefix[b], rem = x0 - prefix[b] * p.Hkv;
@@ -839,15 +842,15 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   cell_prefix<MW * 32>(p, prefix, nullptr, s_warp);  // decode_k lets this grid start only once the lengths are there
-  const Ranges rg(prefix[p.B] * p.Hkv, p.ranges);
-  const int wpc = rg.per_cta(gridDim.x), end = min(rg.lo((blockIdx.x + 1) * wpc), prefix[p.B] * p.Hkv);  // of CTA i's cells
+  const Ranges rg(prefix[p.B] * p.Hkv, gridDim.x);
+  const int end = min(rg.lo(rg.first(blockIdx.x + 1)), prefix[p.B] * p.Hkv);  // of CTA i's cells
   int n = 0;  // CTAs that the pair that goes on lies in
   bf16* out = nullptr;
   if (end > 0 && end < prefix[p.B] * p.Hkv) {
     const int b = sequence_of(prefix, p.B, (end - 1) / p.Hkv, lane), pc = prefix[b + 1] - prefix[b];
     const int hk = (end - 1 - prefix[b] * p.Hkv) / pc, x0 = prefix[b] * p.Hkv + hk * pc + 1, last = x0 + pc - 3;
-    if (x0 < end && last >= end && rg.of(x0) >= (int)blockIdx.x * wpc) {
-      n = rg.of(last) / wpc - (int)blockIdx.x + 1;
+    if (x0 < end && last >= end && rg.of(x0) >= rg.first(blockIdx.x)) {
+      n = rg.cta_of(rg.of(last)) - (int)blockIdx.x + 1;
       out = p.out + ((long)b * p.Hkv + hk) * p.G * D;
     }
   }
@@ -1013,7 +1016,7 @@ at::Tensor paged_decode_attn_fp8(const at::Tensor& q_, const at::Tensor& k, cons
   // without merge_k.  The block table bounds the lengths.  32 q and 8 kv heads: one sequence of 300 tokens 6.5 against 8.3 us,
   // 16 of 512 7.2 against 10.1; with more units to a warp the ranges win (one sequence of 2048: 10.0 against 15.3).
   const bool direct = B * c.Hkv <= num_sms() && (long)block_table.size(1) * c.P <= DIRECT_TOKENS;
-  const int G = (int)(Hq / c.Hkv), grid = direct ? (int)B * c.Hkv : num_sms(), ranges = grid * NW;
+  const int G = (int)(Hq / c.Hkv), grid = direct ? (int)B * c.Hkv : num_sms();
   // partials: freed after the launches, so the memory is handed on in stream order (and is the graph's when captured)
   const long joined = (long)grid * 2 * G, kept = G <= 8 ? 0 : (long)grid * NW * G;
   const c10::DataPtr part = c10::cuda::CUDACachingAllocator::get()->allocate((joined * (D + 2) + kept * D) * sizeof(float));
@@ -1022,7 +1025,7 @@ at::Tensor paged_decode_attn_fp8(const at::Tensor& q_, const at::Tensor& k, cons
   while (box < 64 && c.P % (2 * box) == 0) box *= 2;
   const CUtensorMap tk = codes_map(c.k, rows, box), tv = codes_map(c.v, rows, box);
   const DecParams p{(const bf16*)q.data_ptr(), (const int*)block_table.data_ptr(), (const int*)seq_lens.data_ptr(), c.ks, c.vs, (bf16*)out.data_ptr(),
-                    part_o, (float2*)(part_o + joined * D), part_o + joined * (D + 2), ranges, c.pages, (int)B, G, c.Hkv, c.P,
+                    part_o, (float2*)(part_o + joined * D), part_o + joined * (D + 2), c.pages, (int)B, G, c.Hkv, c.P,
                     (int)block_table.size(1), box, (float)(scale * 1.4426950408889634), direct};
   auto kern = G <= 8 ? decode_k<1> : decode_k<2>;
   smem_attr((const void*)kern, 227 * 1024 - 256);
