@@ -792,6 +792,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
     __syncwarp();
     const float4* from = reinterpret_cast<const float4*>(p.part_w + ((long)blockIdx.x * NW + warp) * p.G * D);
     float4* to = reinterpret_cast<float4*>(ring) + p.G * 32;
+#pragma unroll 8
     for (int i = lane; i < p.G * 32; i += 32) to[i] = __ldcg(from + i);
   }
   if (lane == 0) s_head[warp] = head, s_tail[warp] = tail;
@@ -828,11 +829,12 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   }
 }
 
-// The pairs that lie in several CTAs of decode_k (at most one begins in each and goes on): out = the joined partials of
-// those CTAs; zeros for empty sequences.  CTA i looks for the pair that goes on behind CTA i before decode_k has ended; then
-// its MW warps are dealt to the heads of the group and, where those are fewer, to stripes of the partials, whose loads
-// are all in flight at once.  One warp walking the partials of all warps took 42 us for two contexts of 100k, CTAs of
-// eight warps for every pair 6 us, and 5 us for 256 short sequences; this form 2 us.
+// The pairs that lie in several CTAs of decode_k: out = the joined partials of those CTAs; zeros for empty sequences.  CTA i looks
+// for the pair that goes on behind CTA i before decode_k has ended.  The CTAs that a pair goes on behind share its heads;
+// a CTA's MW warps are dealt to its heads and, where those are fewer, to stripes of the partials, whose loads are in flight
+// together.  One warp walking the partials of all warps took 42 us for two contexts of 100k, CTAs of eight warps for every
+// pair 6 us, and 5 us for 256 short sequences; this form 2 us.  With all heads left to the pair's first CTA, two sequences of
+// 1943 tokens with two kv heads (31 CTAs a pair, 16 heads) took 23 us in all, shared 14.
 constexpr int MW = 8, MBATCH = 4;
 
 __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
@@ -845,13 +847,14 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
   cell_prefix<MW * 32>(p, prefix, nullptr, s_warp);  // decode_k lets this grid start only once the lengths are there
   const Ranges rg(prefix[p.B] * p.Hkv, gridDim.x);
   const int end = min(rg.lo(rg.first(blockIdx.x + 1)), prefix[p.B] * p.Hkv);  // of CTA i's cells
-  int n = 0;  // CTAs that the pair that goes on lies in
+  int n = 0, i0 = 0;  // the pair that goes on lies in n CTAs from i0
   bf16* out = nullptr;
   if (end > 0 && end < prefix[p.B] * p.Hkv) {
     const int b = sequence_of(prefix, p.B, (end - 1) / p.Hkv, lane), pc = prefix[b + 1] - prefix[b];
     const int hk = (end - 1 - prefix[b] * p.Hkv) / pc, x0 = prefix[b] * p.Hkv + hk * pc + 1, last = x0 + pc - 3;
-    if (x0 < end && last >= end && rg.of(x0) >= rg.first(blockIdx.x)) {
-      n = rg.cta_of(rg.of(last)) - (int)blockIdx.x + 1;
+    if (x0 < end && last >= end) {
+      i0 = rg.cta_of(rg.of(x0));
+      n = rg.cta_of(rg.of(last)) - i0 + 1;
       out = p.out + ((long)b * p.Hkv + hk) * p.G * D;
     }
   }
@@ -860,17 +863,21 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
     if (prefix[b + 1] == prefix[b])
       for (int i = threadIdx.x; i < p.Hkv * p.G * D / 8; i += MW * 32) reinterpret_cast<uint4*>(p.out + (long)b * p.Hkv * p.G * D)[i] = make_uint4(0, 0, 0, 0);
   if (out == nullptr) return;
-  const int stripes = p.G >= MW ? 1 : MW / p.G, stripe = warp / p.G;  // (a head and a stripe) per warp, heads in turn if G > MW
+  // heads h0, h0 + n - 1, ... of the group: `mine` of them
+  const int h0 = (int)blockIdx.x - i0, mine = h0 < p.G ? (p.G - 1 - h0) / (n - 1) + 1 : 0;
+  if (mine == 0) return;
+  const int stripes = mine >= MW ? 1 : MW / mine, stripe = warp / mine;  // (a head and a stripe) per warp, heads in turn if there are more
   if (stripes == 1 && stripe > 0) return;
-  for (int h = warp % p.G; h < p.G; h += MW) {
+  for (int i = warp % mine; i < mine; i += MW) {
+    const int h = h0 + i * (n - 1);
     Partial y = empty_partial();
     if (stripe < stripes)
       for (int k = stripe; k < n; k += stripes * MBATCH) {
         Partial x[MBATCH + 1];
 #pragma unroll
-        for (int i = 0; i < MBATCH; ++i) {
-          const int at = k + i * stripes;
-          x[i] = at < n ? load_partial(p, (((int)blockIdx.x + at) * 2 + (at == 0)) * p.G + h, lane) : empty_partial();
+        for (int e = 0; e < MBATCH; ++e) {
+          const int at = k + e * stripes;
+          x[e] = at < n ? load_partial(p, ((i0 + at) * 2 + (at == 0)) * p.G + h, lane) : empty_partial();
         }
         x[MBATCH] = y;
         y = join(x);
@@ -878,11 +885,11 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
     if (stripes > 1) {
       s_o[warp][lane] = y.o;
       if (lane == 0) s_ml[warp] = make_float2(y.m, y.l);
-      __syncthreads();  // G < MW: every warp passes here once
+      __syncthreads();  // mine < MW: every warp passes here once
       if (stripe > 0) return;
       for (int k = 1; k < stripes; ++k) {
-        const float2 ml = s_ml[warp + k * p.G];
-        const Partial x[2] = {y, {s_o[warp + k * p.G][lane], ml.x, ml.y}};
+        const float2 ml = s_ml[warp + k * mine];
+        const Partial x[2] = {y, {s_o[warp + k * mine][lane], ml.x, ml.y}};
         y = join(x);
       }
     }
