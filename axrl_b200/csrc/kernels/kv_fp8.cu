@@ -272,7 +272,8 @@ constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 2, TILE = UNIT * D;  // TILE
 constexpr int MAXB = 2048, DIRECT_TOKENS = NW * UNIT;
 constexpr int DEC_FIXED = NW * SLOTS * (TILE + UNIT + 8 + 4);
 // Shared memory of a CTA: rings, scales, barriers, flags; q rows, partials of pairs that began before the warps' ranges (groups of
-// up to eight heads; larger ones keep them in global memory meanwhile), their maxima and sums; cell prefix and lengths.
+// up to eight heads; larger ones keep them in global memory while the ring is in use), their maxima and sums; cell prefix and
+// lengths.
 constexpr int dec_smem(int G, int B) { return 1024 + DEC_FIXED + NW * G * (D * 2 + (G <= 8 ? D * 4 : 0) + 16) + (2 * B + 1) * 4; }
 static_assert(dec_smem(8, MAXB) <= 227 * 1024 - 256 && dec_smem(MAXG, MAXB) <= 227 * 1024 - 256, "shared memory");
 static_assert(2 * MAXG * D * 4 <= SLOTS * TILE, "both partials of a warp fit its ring");
@@ -288,7 +289,7 @@ struct DecParams {
   bf16* out;           // (B, Hq, 128)
   float* part_o;       // (CTAs, 2, G, 128): of the pair that began before the CTA's ranges, of the one that goes on behind them
   float2* part_ml;     // (CTAs, 2, G): max, sum
-  float* part_w;       // (CTAs, NW, G, 128), groups above eight: kept for the warps' first pairs
+  float* part_w;       // (CTAs, NW, G, 128), groups above eight: the warps' first pairs that end before their ranges do
   long pages;
   int B, G, Hkv, P, max_pages, box;  // box: token rows of one TMA load, gcd(P, 64)
   float scale_log2;
@@ -583,7 +584,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   float acc[NT][8][4], m[NT][2], l[NT][2], qs[NT][2];  // columns 2c, 2c + 1 of a tile: heads 8 t + 2 c, + 1
   uint32_t qf[NT][16];
   bool fresh = true, begun_before = u > 0;  // the pair at the start of the range may have begun in an earlier one
-  int j = 0, head = 0, tail = 0;  // a pair that began before this range has a partial; the pair that goes on behind it: 1 if it began before, 2 if in it
+  int j = 0, head = 0, tail = 0;  // a pair that began before this range has a partial (2: it ended before the range did); the pair that goes on behind it: 1 if it began before, 2 if in it
   while (left > 0) {
     const int sk = j % SLOTS, sv = (j + 1) % SLOTS;
     // --- scores of 64 tokens
@@ -751,8 +752,9 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
     left -= ends ? 3 : 2;
     if (ends || left <= 0) {
       const bool whole = ends && !begun_before;
-      // what goes on lies in this warp's ring, whose tiles have all been used by then
-      float* rec = !begun_before ? reinterpret_cast<float*>(ring) : NT == 1 ? s_rec + warp * p.G * D : p.part_w + ((long)blockIdx.x * NW + warp) * p.G * D;
+      // at the end of the range the warp's ring is free: what goes on lies there, and behind it the large groups' first pair
+      float* rec = reinterpret_cast<float*>(ring);
+      if (begun_before) rec = NT == 1 ? s_rec + warp * p.G * D : left <= 0 ? rec + p.G * D : p.part_w + ((long)blockIdx.x * NW + warp) * p.G * D;
       float2* rec_ml = s_ml + (warp * 2 + !begun_before) * p.G;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -774,7 +776,7 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
             if (!whole && g == 0) rec_ml[h] = make_float2(m[t][cc], sum);
           }
         }
-      head |= begun_before;
+      if (begun_before) head = left <= 0 ? 1 : 2;
       if (!ends) {
         tail = begun_before ? 1 : 2;
         if (lane == 0) s_pair[warp] = b * p.Hkv + hk;
@@ -788,12 +790,17 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
   for (; j < nj; ++j) wait_tile(&full[j % SLOTS], (j / SLOTS) & 1);
 
   // Join the partials of pairs that lie in several ranges of this CTA: a warp takes a head and walks the ranges in order.
-  if (NT == 2 && head) {
+  if (NT == 2 && head == 2) {
     __syncwarp();
-    const float4* from = reinterpret_cast<const float4*>(p.part_w + ((long)blockIdx.x * NW + warp) * p.G * D);
-    float4* to = reinterpret_cast<float4*>(ring) + p.G * 32;
-#pragma unroll 8
-    for (int i = lane; i < p.G * 32; i += 32) to[i] = __ldcg(from + i);
+    const float4* from = reinterpret_cast<const float4*>(p.part_w + ((long)blockIdx.x * NW + warp) * p.G * D) + lane;
+    float4* to = reinterpret_cast<float4*>(ring) + p.G * 32 + lane;
+    float4 x[MAXG];
+#pragma unroll
+    for (int h = 0; h < MAXG; ++h)
+      if (h < p.G) x[h] = __ldcg(from + 32 * h);
+#pragma unroll
+    for (int h = 0; h < MAXG; ++h)
+      if (h < p.G) to[32 * h] = x[h];
   }
   if (lane == 0) s_head[warp] = head, s_tail[warp] = tail;
   __syncthreads();
@@ -834,7 +841,8 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
 // a CTA's MW warps are dealt to its heads and, where those are fewer, to stripes of the partials, whose loads are in flight
 // together.  One warp walking the partials of all warps took 42 us for two contexts of 100k, CTAs of eight warps for every
 // pair 6 us, and 5 us for 256 short sequences; this form 2 us.  With all heads left to the pair's first CTA, two sequences of
-// 1943 tokens with two kv heads (31 CTAs a pair, 16 heads) took 23 us in all, shared 14.
+// 1943 tokens with two kv heads (31 CTAs a pair, 16 heads) took 23 us in all, shared 14
+// (11.5 since the large groups' partials stay on the SM).
 constexpr int MW = 8, MBATCH = 4;
 
 __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {

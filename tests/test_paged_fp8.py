@@ -303,7 +303,16 @@ def test_decode_many_short_sequences(B):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("hq,hkv", [(8, 2), (16, 1)])
+@pytest.mark.parametrize("hq,hkv", [(16, 1), (11, 1), (16, 2), (3, 1)])
+def test_decode_ragged_batches(hq, hkv):
+    """Ranges that hold the end of one pair and the start of the next, several short ones, or the middle of a long one."""
+    g = torch.Generator().manual_seed(hq)
+    lens = (torch.rand(120, generator=g) ** 3 * 4000).int().tolist()
+    _check_decode(*_decode_case(lens, hq, hkv, 64, "cuda", seed=hq))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (16, 1), (24, 2)])
 def test_decode_long_context(hq, hkv):
     _check_decode(*_decode_case([70001, 33000], hq, hkv, 64, "cuda"))
 
@@ -492,5 +501,8 @@ def test_refusals():
     _refused(dec, lens=lens.cpu())
     _refused(dec, cache=cache._replace(v=cache.v[:, :, :8]))
     _refused(dec, cache=_cache(3, 2, 24, dev))  # pages are multiples of 16 tokens
+    many = (torch.zeros(2049, 4, D, dtype=torch.bfloat16, device=dev), torch.zeros(2049, 3, dtype=torch.int32, device=dev), torch.ones(2049, dtype=torch.int32, device=dev))
+    _refused(dec, *many[:1], cache, *many[1:])
+    assert dec(many[0][1:], cache, many[1][1:], many[2][1:]).shape == (2048, 4, D)
     assert dec(q=q[:0], bt=bt[:0], lens=lens[:0]).shape == (0, 4, D)
     assert (dec(bt=bt[:, :0]) == 0).all()
