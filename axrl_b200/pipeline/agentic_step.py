@@ -33,7 +33,7 @@ from axrl_b200.data.rollout_trace import RolloutTrace
 from axrl_b200.data.sample import SampleBatch
 from axrl_b200.models.qwen3 import Qwen3Config
 from axrl_b200.pipeline.rewards import group_advantages
-from axrl_b200.rollout.engine import GenRequest, RolloutEngine
+from axrl_b200.rollout.engine import GenRequest, RolloutEngine, kv_token_bytes
 from axrl_b200.train.engine import TrainEngine
 from axrl_b200.trainer.grpo_trainer import GrpoTrainer
 from axrl_b200.utils import iostats
@@ -58,6 +58,7 @@ class AgenticConfig:
     temperature: float = 1.0
     seed: int = 0
     use_cuda_graph: bool = True
+    kv_format: str = "bf16"  # or "fp8_block": 8-bit KV cache, and each turn prefills only what its cached prompt leaves
     kv_gb: float | None = None
     extra: dict = field(default_factory=dict)
 
@@ -85,12 +86,11 @@ class SyntheticAgentic:
         n_seq = ac.inflight_groups * ac.group_size
         kv_tokens = n_seq * (ac.max_context + 64)
         if ac.kv_gb is not None:
-            per_tok = 2 * model_cfg.num_hidden_layers * model_cfg.num_key_value_heads * model_cfg.head_dim * 2
-            kv_tokens = min(kv_tokens, int(ac.kv_gb * (1 << 30)) // per_tok)
+            kv_tokens = min(kv_tokens, int(ac.kv_gb * (1 << 30)) // kv_token_bytes(model_cfg, ac.kv_format))
         cuda = self.device.type == "cuda"
         self.rollout = RolloutEngine(self.train.model, max_batch=n_seq, kv_tokens=kv_tokens, page_size=64, max_context=ac.max_context + 8,
                                      max_prefill_tokens=max(16384, ac.prefix_len), seed=ac.seed, use_cuda_graph=ac.use_cuda_graph and cuda,
-                                     eos_token_id=ac.eos_token_id, kv_memory_saver=cuda)
+                                     eos_token_id=ac.eos_token_id, kv_memory_saver=cuda, kv_format=ac.kv_format)
         if cuda and self.train.optim is not None:
             self.train.release_grads_after_step = True
         self.pool: list[list[_Traj]] = []

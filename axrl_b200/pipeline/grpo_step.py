@@ -38,7 +38,7 @@ from axrl_b200.data.prefix_tree import merge_trajectory_samples
 from axrl_b200.data.sample import Sample, SampleBatch
 from axrl_b200.models.qwen3 import Qwen3Config
 from axrl_b200.pipeline.rewards import group_advantages
-from axrl_b200.rollout.engine import GenRequest, GenResult, RolloutEngine
+from axrl_b200.rollout.engine import GenRequest, GenResult, RolloutEngine, kv_token_bytes
 from axrl_b200.train.engine import TrainEngine
 from axrl_b200.trainer.grpo_trainer import GrpoTrainer
 from axrl_b200.utils import iostats
@@ -74,6 +74,7 @@ class SyntheticGRPOConfig:
     max_batch: int | None = None
     use_cuda_graph: bool = True
     kv_gb: float | None = None  # cap on the KV pool size
+    kv_format: str = "bf16"  # or "fp8_block": the rollout engine's 8-bit KV cache
     kv_memory_saver: bool = True  # release the KV pool while training (same address on resume)
     partial_rollout: bool = False  # keep unfinished groups in flight across steps
     inflight_prompts: int | None = None  # groups in flight with partial rollout (default 2 x num_prompts)
@@ -128,8 +129,7 @@ class SyntheticGRPO:
         kv_tokens = sc.kv_tokens or n_seq * (-(-max_ctx // 64) * 64)
         cuda = self.device.type == "cuda"
         if sc.kv_gb is not None:
-            per_tok = 2 * model_cfg.num_hidden_layers * model_cfg.num_key_value_heads * model_cfg.head_dim * 2
-            kv_tokens = min(kv_tokens, int(sc.kv_gb * (1 << 30)) // per_tok)
+            kv_tokens = min(kv_tokens, int(sc.kv_gb * (1 << 30)) // kv_token_bytes(model_cfg, sc.kv_format))
         # tensor parallelism: the rollout engine runs on the trainer's own shards (same TP layout) and
         # needs the whole embedding table, gathered from the vocabulary shards after every update
         tp = self.train.tp
@@ -141,7 +141,7 @@ class SyntheticGRPO:
         self.rollout = RolloutEngine(rollout_model, max_batch=sc.max_batch or n_seq, kv_tokens=kv_tokens, page_size=64,
                                      max_context=max_ctx, max_prefill_tokens=max(16384, sc.prompt_len), seed=sc.seed,
                                      use_cuda_graph=sc.use_cuda_graph, eos_token_id=sc.eos_token_id,
-                                     kv_memory_saver=cuda and sc.kv_memory_saver,
+                                     kv_memory_saver=cuda and sc.kv_memory_saver, kv_format=sc.kv_format,
                                      dp_attention=_ep_active(rollout_model),
                                      tp_group=self.train.par.tp_group if tp.enabled else None, embed_full=self.embed_full)
         if cuda and self.train.optim is not None:

@@ -112,6 +112,12 @@ class _Seq:
     lslot: int = -1  # slot of its linear-attention (Gated DeltaNet) states, hybrid models
 
 
+def kv_token_bytes(cfg: Any, kv_format: str = "bf16") -> int:
+    """Bytes that one token takes in the KV cache (all layers, K and V)."""
+    row = cfg.head_dim + 1 if kv_format == "fp8_block" else 2 * cfg.head_dim
+    return 2 * cfg.num_hidden_layers * cfg.num_key_value_heads * row
+
+
 def _stream_id(rid: str) -> int:
     return zlib.crc32(rid.encode()) & 0x7FFFFFFF
 

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 
-def build_worker(preset: str, device: str, hf_dir: str | None, max_batch: int, max_context: int, seed: int):  # noqa: ANN201
+def build_worker(preset: str, device: str, hf_dir: str | None, max_batch: int, max_context: int, seed: int, kv_format: str = "bf16"):  # noqa: ANN201
     from axrl_b200.configs import SamplingConfig
     from axrl_b200.models.qwen3 import Qwen3Model, resolve_preset
     from axrl_b200.rollout.engine import RolloutEngine
@@ -37,7 +37,7 @@ def build_worker(preset: str, device: str, hf_dir: str | None, max_batch: int, m
     for p in model.parameters():
         p.requires_grad_(False)
     engine = RolloutEngine(model, max_batch=max_batch, kv_tokens=max_batch * max_context, max_context=max_context, seed=seed,
-                           use_cuda_graph=device.startswith("cuda"))
+                           use_cuda_graph=device.startswith("cuda"), kv_format=kv_format)
     worker = RolloutWorker(engine, SamplingConfig())
 
     @torch.no_grad()
@@ -68,12 +68,13 @@ def main(argv: list[str] | None = None) -> None:
     ap.add_argument("--max-batch", type=int, default=64)
     ap.add_argument("--max-context", type=int, default=4096)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--kv", default="bf16", choices=["bf16", "fp8_block"], help="KV cache format")
     a = ap.parse_args(argv)
     import uvicorn
 
     from axrl_b200.worker.oai_client import create_generate_app
 
-    worker, teacher = build_worker(a.preset, a.device, a.hf_dir, a.max_batch, a.max_context, a.seed)
+    worker, teacher = build_worker(a.preset, a.device, a.hf_dir, a.max_batch, a.max_context, a.seed, a.kv)
     uvicorn.run(create_generate_app(worker, teacher_model=teacher), host=a.host, port=a.port, log_level="warning")
 
 

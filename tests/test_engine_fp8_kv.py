@@ -167,3 +167,46 @@ def test_shapes_without_kernels_are_refused():
         _engine(m, "cuda", page_size=24)
     with pytest.raises(ValueError, match="fp8_block"):
         _engine(m, "cuda", max_batch=4096)
+
+
+def test_token_bytes():
+    from axrl_b200.rollout.engine import kv_token_bytes
+
+    cfg = _model("cpu").cfg
+    codes, scales = _engine(_model("cpu"), "cpu").kv_fp8
+    rows = codes.numel() // 128
+    assert kv_token_bytes(cfg, "fp8_block") * (codes.shape[2] * codes.shape[4]) == codes.numel() + scales.numel() == rows * 129
+    assert kv_token_bytes(cfg) == 2 * 2 * 2 * 128 * 2
+
+
+def test_agentic_turns_continue_cached_prefixes():
+    """Each turn of a trajectory begins with the context of the one before: on the 8-bit cache it prefills less."""
+    from axrl_b200.configs import GrpoTrainerConfig, MegatronWorkerConfig
+    from axrl_b200.models.qwen3 import resolve_preset
+    from axrl_b200.pipeline.agentic_step import AgenticConfig, SyntheticAgentic
+
+    done = {}
+    for kv in ("bf16", "fp8_block"):
+        torch.manual_seed(0)
+        ac = AgenticConfig(group_size=2, inflight_groups=1, prefix_len=80, min_turns=3, max_turns=3, action_min=4, action_max=4, obs_min=70, obs_max=70,
+                           max_context=400, pack_len=1024, seed=1, kv_format=kv, kv_gb=0.01)
+        pipe = SyntheticAgentic(resolve_preset("tiny"), MegatronWorkerConfig(), GrpoTrainerConfig(loss_type="grpo"), ac, "cpu")
+        m = pipe.run_step()
+        assert m["trajectories"] == 2 and m["turns"] == 6
+        done[kv] = pipe.rollout.stats["prefill_tokens"]
+    assert done["fp8_block"] < done["bf16"]
+
+
+@pytest.mark.gpu
+def test_grpo_step_on_the_8_bit_cache():
+    from axrl_b200.configs import GrpoTrainerConfig, MegatronWorkerConfig
+    from axrl_b200.pipeline.grpo_step import SyntheticGRPO, SyntheticGRPOConfig
+
+    wc = MegatronWorkerConfig()
+    wc.lr_scheduler.lr_warmup_steps = 0
+    sc = SyntheticGRPOConfig(num_prompts=2, prompt_len=64, group_size=4, max_new_tokens=24, reward_token=5, kv_format="fp8_block")
+    g = SyntheticGRPO(_model("cpu").cfg, wc, GrpoTrainerConfig(loss_type="grpo"), sc, "cuda")
+    for _ in range(2):
+        m = g.run_step()
+        assert m["trained_tokens"] > 0 and m["loss"] == m["loss"]
+    g.rollout.release_graphs()
