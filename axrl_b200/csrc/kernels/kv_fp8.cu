@@ -263,12 +263,19 @@ __global__ void __launch_bounds__(256) load_k(Cache c, const int64_t* __restrict
 // clk for the load, conversions and two products above, which serve twice the heads (256 short sequences with groups of
 // eight: 56.5 us against 40.4).
 //
-// Softmax in the log2 domain on w_t = scale log2(e) q.k_t + e_t, the exponent of V folded in: P_t = 2^{w_t - max w} <= 1
-// rounds to f16 (2^-11, finer than bf16) and multiplies the codes themselves, and the normaliser is l = sum P_t 2^{-e_t}
-// in fp32, unrounded.  Whatever falls below f16 is 2^-24 of the largest weighted term; P itself leaves fp32 (and l) only where
-// exponents of V in a sequence lie 100 and more apart, which scales of at least 2^-60 do not below |v| = 10^14.  q rows are scaled by a power of
-// two so that their largest is in [2^14, 2^15) and round to f16 exactly but for what is below 2^-28 of it.
+// Softmax in the log2 domain on w_t = scale log2(e) q.k_t + e_t, the exponent of V folded in: P_t = 2^{w_t - max w + HEAD}
+// rounds to f16 (2^-11, finer than bf16) and multiplies the codes themselves, and the normaliser is l = sum P_t 2^{-e_t} in
+// fp32, unrounded. HEAD = 15 uses f16 up to 2^15: a weight is rounded in full down to 2^-29 of the largest and is off by at
+// most 2^-40 of it below, so that a row whose codes are as small as codes get (2^-9 of 2^9) may have the largest weight and the
+// others still keep what they add. A row of zeros adds nothing at any weight: it is weighed as if its scale were the smallest
+// that append writes, 2^-60 (with its own it would set the maximum and push the rows that do add something out of f16: with one
+// of 2^0, 8 above the others' scores, the outputs of 300 tokens of values of size 10^-3 were off by 35 % of the largest;
+// telling such rows costs 0 to 1 % of the time). P itself leaves fp32 (and l) only where exponents of V in a sequence lie 100
+// and more apart, which scales of at least 2^-60 do not below |v| = 10^14; l holds 10^6 rows of scales down to 2^-90. q rows
+// are scaled by a power of two so that their largest is in [2^14, 2^15) and round to f16 exactly but for what is below 2^-28 of
+// it.
 constexpr int MAXG = 16, UNIT = 64, NW = 8, SLOTS = 2, TILE = UNIT * D;  // TILE: bytes of one slot
+constexpr float HEAD = 15.f;
 constexpr int MAXB = 2048, DIRECT_TOKENS = NW * UNIT;
 constexpr int DEC_FIXED = NW * SLOTS * (TILE + UNIT + 8 + 4);
 // Shared memory of a CTA: rings, scales, barriers, flags; q rows, partials of pairs that began before the warps' ranges (groups of
@@ -360,6 +367,26 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ void bulk_bytes(void* dst, const void* src, int bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::s32(dst)), "l"(src), "r"(bytes), "r"(tc::s32(bar))
                : "memory");
+}
+
+// Four codes of row `lane` and four of row 32 + lane of a tile, each lane's from a bank of its own: 0 if one of the two rows may be
+// a row of zeros (-0 is a zero too).
+constexpr uint32_t MAGNITUDES = 0x7f7f7f7fu;
+__device__ __forceinline__ uint32_t first_look(const char* tile, int lane) {
+  const char* at = tile + lane * D + (lane & 7) * 16 + (lane >> 3) * 4;
+  return min(*reinterpret_cast<const uint32_t*>(at) & MAGNITUDES, *reinterpret_cast<const uint32_t*>(at + 32 * D) & MAGNITUDES);
+}
+// The tile's rows of zeros, a bit a row.  All lanes of a warp; apart from the loop around it, which hardly ever comes here.
+__device__ __noinline__ uint64_t zero_rows(const char* tile) {
+  const int lane = threadIdx.x & 31;
+  uint32_t a = 0, b = 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const uint4* at = reinterpret_cast<const uint4*>(tile + lane * D + ((i ^ lane) & 7) * 16);
+    const uint4 x = at[0], y = at[32 * D / 16];
+    a |= x.x | x.y | x.z | x.w, b |= y.x | y.y | y.z | y.w;
+  }
+  return __ballot_sync(0xffffffffu, (a & MAGNITUDES) == 0u) | (uint64_t)__ballot_sync(0xffffffffu, (b & MAGNITUDES) == 0u) << 32;
 }
 
 // Position of a warp's loads in its range.
@@ -654,8 +681,9 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
     }
     __syncwarp();
     load_next();
-    // --- w = scale log2(e) q.k + e, and P = 2^{w - max w}
+    // --- w = scale log2(e) q.k + e, and P = 2^{w - max w + HEAD}
     if (!__all_sync(0xffffffffu, wait_tile(&full[sv], ((j + 1) / SLOTS) & 1))) break;
+    const uint32_t look = first_look(ring + sv * TILE, lane);
     uint64_t seen = ~0ull;  // tokens of the unit that count
     if (partial) {
       seen = 0;
@@ -676,6 +704,19 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) s[t][i16][2 * hh + cc] = fmaf(s[t][i16][2 * hh + cc], qs[t][cc], e);
       }
+    if (__any_sync(0xffffffffu, look == 0u)) {
+      const uint64_t zero = zero_rows(ring + sv * TILE);
+#pragma unroll
+      for (int i16 = 0; i16 < 4; ++i16)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+          if (zero >> (i16 * 16 + (hh ? tok_b : tok_a)) & 1) {  // e becomes -60; a row that is not finite stays NaN
+            const float to = (float)((int)(__float_as_uint(inv[i16][hh]) >> 23) - 127 - 60);
+            inv[i16][hh] = 0x1p60f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[t][i16][2 * hh] += to, s[t][i16][2 * hh + 1] += to;
+          }
+    }
     if (partial) {
 #pragma unroll
       for (int i16 = 0; i16 < 4; ++i16)
@@ -697,7 +738,8 @@ __global__ void __maxnreg__(192) decode_k(const __grid_constant__ CUtensorMap tk
         for (int i16 = 1; i16 < 4; ++i16) mx = fmaxf(mx, fmaxf(s[t][i16][cc], s[t][i16][2 + cc]));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        mx = fmaxf(m[t][cc], mx);
+        // m: HEAD below the largest w, where the difference is exact to far less than the headroom above 2^15
+        mx = fmaxf(m[t][cc], fabsf(mx) < 0x1p20f ? mx - HEAD : mx);
         ref[cc] = mx == -INFINITY ? 0.f : mx;  // nothing seen yet
         alpha[cc] = ex2(m[t][cc] - ref[cc]);
         m[t][cc] = mx;

@@ -149,7 +149,8 @@ def decode_attention_fp8_ref(q: torch.Tensor, cache: Fp8KV, block_table: torch.T
 def paged_decode_attention_fp8(q: torch.Tensor, cache: Fp8KV, block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float | None = None) -> torch.Tensor:
     """One query token per sequence, ``q (B, Hq, 128)``, over the first ``seq_lens[b]`` tokens of its pages
     ``block_table[b]`` (int32).  GQA groups up to 16, up to 2048 sequences, pages of a multiple of 16 tokens.  A length of 0 gives zeros; lengths beyond the block table are cut to
-    it; tokens of a page id outside the cache are not seen.  Needs no plan and no workspace of the caller's."""
+    it; tokens of a page id outside the cache are not seen.  A value row of zeros may have any scale; the scales of the others are at
+    least 2^-90 (append writes none below 2^-60).  Needs no plan and no workspace of the caller's."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if not q.is_cuda:
         return decode_attention_fp8_ref(q, cache, block_table, seq_lens, scale)
