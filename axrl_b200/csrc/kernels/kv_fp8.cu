@@ -1095,10 +1095,12 @@ at::Tensor paged_decode_attn_fp8(const at::Tensor& q_, const at::Tensor& k, cons
   return out;
 }
 
-// 0, or the code of the first bounded wait of the decode kernel that gave up on the current device.
+// 0, or the code of the first bounded wait of the decode kernel that gave up on the current device, in what the current stream
+// was given so far; waits for that.
 int64_t kv_fp8_error() {
   int v = 0;
-  AX_CUDA_OK(cudaMemcpyFromSymbol(&v, kv8::g_decode_err, sizeof(int)));
+  AX_CUDA_OK(cudaMemcpyFromSymbolAsync(&v, kv8::g_decode_err, sizeof(int), 0, cudaMemcpyDeviceToHost, stream()));
+  AX_CUDA_OK(cudaStreamSynchronize(stream()));
   return v;
 }
 

@@ -150,8 +150,25 @@ def paged_decode_attention_fp8(q: torch.Tensor, cache: Fp8KV, block_table: torch
     """One query token per sequence, ``q (B, Hq, 128)``, over the first ``seq_lens[b]`` tokens of its pages
     ``block_table[b]`` (int32).  GQA groups up to 16, up to 2048 sequences, pages of a multiple of 16 tokens.  A length of 0 gives zeros; lengths beyond the block table are cut to
     it; tokens of a page id outside the cache are not seen.  A value row of zeros may have any scale; the scales of the others are at
-    least 2^-90 (append writes none below 2^-60).  Needs no plan and no workspace of the caller's."""
+    least 2^-90 (append writes none below 2^-60).  Needs no plan and no workspace of the caller's.  After a
+    wait inside the kernel that gave up, rows may be undefined: :func:`check_decode_waits` tells."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if not q.is_cuda:
         return decode_attention_fp8_ref(q, cache, block_table, seq_lens, scale)
     return _ext.ext().paged_decode_attn_fp8(q, *cache, block_table, seq_lens, scale)
+
+
+def decode_wait_error(device: torch.device) -> int:
+    """0, or the code of the first wait inside :func:`paged_decode_attention_fp8` that gave up on ``device`` since the process
+    started.  Waits for the current stream."""
+    if device.type != "cuda":
+        return 0
+    with torch.cuda.device(device):
+        return int(_ext.ext().kv_fp8_error())
+
+
+def check_decode_waits(device: torch.device) -> None:
+    """Raise if a wait inside the decode attention gave up on ``device``: its outputs are then incomplete."""
+    code = decode_wait_error(device)
+    if code:
+        raise RuntimeError(f"decode attention over the 8-bit KV cache: a wait inside the kernel timed out (code {code}) on {device}")

@@ -884,6 +884,8 @@ class RolloutEngine:
                         captured_rows.append(np.stack([capture[li][:B].cpu().numpy() for li in sorted(capture)], 1))
         toks = self.ring_tok[:k, :B].cpu()
         lps = self.ring_lp[:k, :B].cpu()
+        if self.kv_fp8 is not None:  # before a token of this burst is used
+            paged_fp8.check_decode_waits(self.device)
         if self.is_cuda:
             iostats.add_d2h(self.ring_tok[:k, :B], self.ring_lp[:k, :B])
         toks_l, lps_l = toks.T.tolist(), lps.T.tolist()
