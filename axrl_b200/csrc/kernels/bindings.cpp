@@ -119,6 +119,7 @@ std::tuple<at::Tensor, at::Tensor> gather_kv_fp8(const at::Tensor& k, const at::
                                                  const at::Tensor& slots, const c10::optional<at::Tensor>& out_k, const c10::optional<at::Tensor>& out_v);
 at::Tensor paged_decode_attn_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
                                  const at::Tensor& block_table, const at::Tensor& seq_lens, double scale);
+int64_t paged_decode_attn_fp8_launches(int64_t B, int64_t pages, int64_t Hkv, int64_t P, int64_t max_pages);
 int64_t kv_fp8_error();
 }  // namespace ax
 
@@ -226,5 +227,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qknorm_rope_cache_fp8", &ax::qknorm_rope_cache_fp8);
   m.def("gather_kv_fp8", &ax::gather_kv_fp8);
   m.def("paged_decode_attn_fp8", &ax::paged_decode_attn_fp8);
+  m.def("paged_decode_attn_fp8_launches", &ax::paged_decode_attn_fp8_launches);
   m.def("kv_fp8_error", &ax::kv_fp8_error);
 }

@@ -947,6 +947,11 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
   }
 }
 
+// Few short sequences: a CTA per (sequence, kv head), a unit per warp at most, does without the prefix over the lengths and
+// without merge_k.  The block table bounds the lengths.  32 q and 8 kv heads: one sequence of 300 tokens 6.5 against 8.3 us,
+// 16 of 512 7.2 against 10.1; with more units to a warp the ranges win (one sequence of 2048: 10.0 against 15.3).
+static bool direct_path(int64_t B, int64_t Hkv, int64_t P, int64_t max_pages) { return B * Hkv <= num_sms() && max_pages * P <= DIRECT_TOKENS; }
+
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 // A cache tensor as (pages Hkv P) rows of 128 codes; boxes of `box` rows, 128-byte swizzle.
@@ -1070,10 +1075,7 @@ at::Tensor paged_decode_attn_fp8(const at::Tensor& q_, const at::Tensor& k, cons
   auto out = empty_bf16({B, Hq, D}, dev);
   if (B == 0) return out;
   if (rows == 0 || block_table.size(1) == 0) return out.zero_();
-  // Few short sequences: a CTA per (sequence, kv head), a unit per warp at most, does without the prefix over the lengths and
-  // without merge_k.  The block table bounds the lengths.  32 q and 8 kv heads: one sequence of 300 tokens 6.5 against 8.3 us,
-  // 16 of 512 7.2 against 10.1; with more units to a warp the ranges win (one sequence of 2048: 10.0 against 15.3).
-  const bool direct = B * c.Hkv <= num_sms() && (long)block_table.size(1) * c.P <= DIRECT_TOKENS;
+  const bool direct = direct_path(B, c.Hkv, c.P, block_table.size(1));
   const int G = (int)(Hq / c.Hkv), grid = direct ? (int)B * c.Hkv : num_sms();
   // partials: freed after the launches, so the memory is handed on in stream order (and is the graph's when captured)
   const long joined = (long)grid * 2 * G, kept = G <= 8 ? 0 : (long)grid * NW * G;
@@ -1093,6 +1095,12 @@ at::Tensor paged_decode_attn_fp8(const at::Tensor& q_, const at::Tensor& k, cons
   launch_pdl(merge_k, dim3(grid), dim3(MW * 32), (B + 1) * sizeof(int), stream(), p);
   AX_LAUNCH_OK();
   return out;
+}
+
+// Kernels that paged_decode_attn_fp8 launches for these sizes.
+int64_t paged_decode_attn_fp8_launches(int64_t B, int64_t pages, int64_t Hkv, int64_t P, int64_t max_pages) {
+  if (B == 0 || pages * P == 0 || max_pages == 0) return 0;
+  return kv8::direct_path(B, Hkv, P, max_pages) ? 1 : 2;
 }
 
 // 0, or the code of the first bounded wait of the decode kernel that gave up on the current device, in what the current stream

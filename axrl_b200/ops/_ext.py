@@ -66,8 +66,11 @@ def load(name: str = "_C") -> ModuleType:
     return mod
 
 
-# Kernel launches per extension entry point (entry points not listed launch one kernel).
-_KERNELS_PER_CALL = {"attn_bwd": 3, "paged_decode_attn": 2, "paged_decode_attn_fp8": 2, "rmsnorm_bwd": 2, "logprob_fwd": 1, "gemm": 1, "sample_tokens": 2}
+# Kernel launches per extension entry point (entry points not listed launch one kernel); a function of the module and the call's
+# arguments where the sizes decide.
+_KERNELS_PER_CALL = {"attn_bwd": 3, "paged_decode_attn": 2,
+                     "paged_decode_attn_fp8": lambda mod, q, k, v, ks, vs, bt, *_: mod.paged_decode_attn_fp8_launches(q.shape[0], *k.shape[:3], bt.shape[1]),
+                     "rmsnorm_bwd": 2, "logprob_fwd": 1, "gemm": 1, "sample_tokens": 2}
 _COUNT = {"launches": 0, "enabled": False}
 
 
@@ -83,9 +86,11 @@ class _Counting:
             return fn
 
         def wrapped(*a, **k):  # noqa: ANN002, ANN003, ANN202
+            out = fn(*a, **k)
             if _COUNT["enabled"]:
-                _COUNT["launches"] += _KERNELS_PER_CALL.get(name, 1)
-            return fn(*a, **k)
+                n = _KERNELS_PER_CALL.get(name, 1)
+                _COUNT["launches"] += n(self._mod, *a) if callable(n) else n
+            return out
 
         self.__dict__[name] = wrapped  # looked up without __getattr__ from now on
         return wrapped
