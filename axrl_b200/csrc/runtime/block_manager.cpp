@@ -8,13 +8,17 @@
 // registered in the prefix cache under a chained content hash
 //     h_i = mix(h_{i-1}, tokens[i*P .. (i+1)*P))
 // so a later request whose prompt starts with the same tokens reuses the page instead of
-// recomputing it.  Cached pages whose refcount drops to zero stay resident on an LRU list
-// and are evicted only when the free list runs dry.
+// recomputing it.  The hash only finds the page: its tokens are compared, and the page before it
+// must be the one that this content follows, so prompts whose hashes are equal never share pages
+// (the later one is not registered while the earlier one is).  Cached pages whose refcount drops
+// to zero stay resident on an LRU list and are evicted only when the free list runs dry.
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <list>
+#include <memory>
 #include <stdexcept>
 #include <unordered_map>
 #include <vector>
@@ -34,7 +38,7 @@ static inline uint64_t mix64(uint64_t h, uint64_t v) {
 class BlockManager {
  public:
   BlockManager(int64_t num_pages, int64_t page_size)
-      : page_size_(page_size), ref_(num_pages, 0), hash_of_(num_pages, 0), cached_(num_pages, false), lru_pos_(num_pages) {
+      : page_size_(page_size), ref_(num_pages, 0), node_of_(num_pages, nullptr), lru_pos_(num_pages) {
     if (num_pages <= 0 || page_size <= 0) throw std::invalid_argument("num_pages and page_size must be positive");
     free_.reserve(num_pages);
     for (int64_t i = num_pages - 1; i >= 0; --i) free_.push_back((int32_t)i);
@@ -45,7 +49,7 @@ class BlockManager {
   // pages obtainable right now (free + evictable cached)
   int64_t num_available() const { return (int64_t)free_.size() + (int64_t)lru_.size(); }
   int64_t num_free() const { return (int64_t)free_.size(); }
-  int64_t num_cached() const { return (int64_t)index_.size(); }
+  int64_t num_cached() const { return cached_; }
 
   std::vector<int32_t> allocate(int64_t n) {
     if (n > num_available()) throw std::runtime_error("KV cache out of pages");
@@ -64,7 +68,7 @@ class BlockManager {
   void incref(const std::vector<int32_t>& pages) {
     for (int32_t p : pages) {
       check(p);
-      if (ref_[p] == 0 && cached_[p]) lru_.erase(lru_pos_[p]);
+      if (ref_[p] == 0 && node_of_[p]) lru_.erase(lru_pos_[p]);
       ++ref_[p];
     }
   }
@@ -74,7 +78,7 @@ class BlockManager {
       check(p);
       if (ref_[p] <= 0) throw std::runtime_error("double free of KV page");
       if (--ref_[p] == 0) {
-        if (cached_[p]) {
+        if (node_of_[p]) {
           lru_.push_back(p);
           lru_pos_[p] = std::prev(lru_.end());
         } else {
@@ -89,12 +93,14 @@ class BlockManager {
   std::pair<std::vector<int32_t>, int64_t> match_prefix(const std::vector<int64_t>& tokens) {
     std::vector<int32_t> pages;
     uint64_t h = 0;
+    const Node* at = nullptr;
     int64_t full = (int64_t)tokens.size() / page_size_;
     for (int64_t i = 0; i < full; ++i) {
       h = page_hash(h, tokens, i);
-      auto it = index_.find(h);
-      if (it == index_.end()) break;
-      pages.push_back(it->second);
+      auto it = nodes_.find(h);
+      if (it == nodes_.end() || it->second->page < 0 || !holds(*it->second, at, tokens, i)) break;
+      at = it->second.get();
+      pages.push_back(at->page);
     }
     incref(pages);
     ++lookups_;
@@ -106,25 +112,34 @@ class BlockManager {
   void insert(const std::vector<int64_t>& tokens, const std::vector<int32_t>& pages) {
     uint64_t h = 0;
     int64_t full = std::min<int64_t>((int64_t)tokens.size() / page_size_, (int64_t)pages.size());
+    for (int64_t i = 0; i < full; ++i) check(pages[i]);
+    Node* at = nullptr;
     for (int64_t i = 0; i < full; ++i) {
       h = page_hash(h, tokens, i);
+      auto it = nodes_.find(h);
+      if (it == nodes_.end()) {
+        std::unique_ptr<Node> n(new Node{at, h, {tokens.begin() + i * page_size_, tokens.begin() + (i + 1) * page_size_}, -1, 0});
+        it = nodes_.emplace(h, std::move(n)).first;
+        if (at) ++at->children;
+      } else if (!holds(*it->second, at, tokens, i)) {
+        break;  // other content with this hash: what follows hangs on this page and is not registered either
+      }
+      at = it->second.get();
       int32_t p = pages[i];
-      check(p);
-      if (index_.count(h) || cached_[p]) continue;
-      index_[h] = p;
-      hash_of_[p] = h;
-      cached_[p] = true;
+      if (at->page >= 0 || node_of_[p]) continue;
+      at->page = p;
+      node_of_[p] = at;
+      ++cached_;
     }
+    trim(at);
   }
 
   void clear_cache() {
-    for (int32_t p : lru_) {
-      cached_[p] = false;
-      free_.push_back(p);
-    }
+    for (int32_t p : lru_) free_.push_back(p);
     lru_.clear();
-    for (auto& kv : index_) cached_[kv.second] = false;
-    index_.clear();
+    std::fill(node_of_.begin(), node_of_.end(), nullptr);
+    nodes_.clear();
+    cached_ = 0;
   }
 
   py::dict stats() const {
@@ -139,6 +154,26 @@ class BlockManager {
   }
 
  private:
+  // Content of a cached page: its tokens behind those of `parent`.  A node outlives its page (page < 0)
+  // as long as nodes hang on it.
+  struct Node {
+    Node* parent;
+    uint64_t hash;
+    std::vector<int64_t> tokens;
+    int32_t page;
+    int64_t children;
+  };
+  bool holds(const Node& n, const Node* parent, const std::vector<int64_t>& t, int64_t i) const {
+    return n.parent == parent && std::equal(n.tokens.begin(), n.tokens.end(), t.begin() + i * page_size_);
+  }
+  void trim(Node* n) {
+    while (n && n->page < 0 && n->children == 0) {
+      Node* up = n->parent;
+      nodes_.erase(n->hash);
+      if (up) --up->children;
+      n = up;
+    }
+  }
   uint64_t page_hash(uint64_t h, const std::vector<int64_t>& t, int64_t i) const {
     for (int64_t j = i * page_size_; j < (i + 1) * page_size_; ++j) h = mix64(h, (uint64_t)t[j]);
     return mix64(h, 0xC0FFEEull + (uint64_t)i);
@@ -150,20 +185,22 @@ class BlockManager {
     if (lru_.empty()) throw std::runtime_error("KV cache out of pages");
     int32_t p = lru_.front();
     lru_.pop_front();
-    index_.erase(hash_of_[p]);
-    cached_[p] = false;
+    Node* n = node_of_[p];
+    node_of_[p] = nullptr;
+    n->page = -1;
+    --cached_;
+    trim(n);
     free_.push_back(p);
   }
 
   int64_t page_size_;
   std::vector<int32_t> ref_;
-  std::vector<uint64_t> hash_of_;
-  std::vector<bool> cached_;
+  std::vector<Node*> node_of_;  // of a cached page
   std::vector<std::list<int32_t>::iterator> lru_pos_;
   std::vector<int32_t> free_;
   std::list<int32_t> lru_;
-  std::unordered_map<uint64_t, int32_t> index_;
-  int64_t lookups_ = 0, hit_tokens_ = 0;
+  std::unordered_map<uint64_t, std::unique_ptr<Node>> nodes_;
+  int64_t cached_ = 0, lookups_ = 0, hit_tokens_ = 0;
 };
 
 void bind_block_manager(py::module_& m) {

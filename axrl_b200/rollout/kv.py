@@ -41,6 +41,18 @@ def _mix64(h: int, v: int) -> int:
     return z ^ (z >> 31)
 
 
+class _Node:
+    """Content of a cached page: its tokens behind those of ``parent``; outlives its page (``page < 0``) as long as nodes hang on it."""
+
+    __slots__ = ("parent", "hash", "tokens", "page", "children")
+
+    def __init__(self, parent: _Node | None, h: int, tokens: list[int]) -> None:
+        self.parent, self.hash, self.tokens, self.page, self.children = parent, h, tokens, -1, 0
+
+    def holds(self, parent: _Node | None, tokens: list[int]) -> bool:
+        return self.parent is parent and self.tokens == list(tokens)
+
+
 class PyBlockManager:
     """Pure-Python twin of the native BlockManager (identical hashing and eviction order)."""
 
@@ -49,9 +61,8 @@ class PyBlockManager:
         self.ref = [0] * num_pages
         self.free = list(range(num_pages - 1, -1, -1))
         self.lru: OrderedDict[int, None] = OrderedDict()
-        self.index: dict[int, int] = {}
-        self.hash_of = [0] * num_pages
-        self.cached = [False] * num_pages
+        self.nodes: dict[int, _Node] = {}
+        self.node_of: list[_Node | None] = [None] * num_pages
 
     def num_available(self) -> int:
         return len(self.free) + len(self.lru)
@@ -60,7 +71,7 @@ class PyBlockManager:
         return len(self.free)
 
     def num_cached(self) -> int:
-        return len(self.index)
+        return sum(n is not None for n in self.node_of)
 
     def allocate(self, n: int) -> list[int]:
         if n > self.num_available():
@@ -69,8 +80,9 @@ class PyBlockManager:
         for _ in range(n):
             if not self.free:
                 p, _ = self.lru.popitem(last=False)
-                del self.index[self.hash_of[p]]
-                self.cached[p] = False
+                node, self.node_of[p] = self.node_of[p], None
+                node.page = -1
+                self._trim(node)
                 self.free.append(p)
             p = self.free.pop()
             self.ref[p] = 1
@@ -79,7 +91,7 @@ class PyBlockManager:
 
     def incref(self, pages: list[int]) -> None:
         for p in pages:
-            if self.ref[p] == 0 and self.cached[p]:
+            if self.ref[p] == 0 and self.node_of[p]:
                 del self.lru[p]
             self.ref[p] += 1
 
@@ -89,7 +101,7 @@ class PyBlockManager:
                 raise RuntimeError("double free of KV page")
             self.ref[p] -= 1
             if self.ref[p] == 0:
-                if self.cached[p]:
+                if self.node_of[p]:
                     self.lru[p] = None
                 else:
                     self.free.append(p)
@@ -99,35 +111,51 @@ class PyBlockManager:
             h = _mix64(h, t[j] & ((1 << 64) - 1))
         return _mix64(h, 0xC0FFEE + i)
 
+    def _trim(self, n: _Node | None) -> None:
+        while n is not None and n.page < 0 and n.children == 0:
+            del self.nodes[n.hash]
+            n = n.parent
+            if n is not None:
+                n.children -= 1
+
     def match_prefix(self, tokens: list[int]) -> tuple[list[int], int]:
-        pages, h = [], 0
-        for i in range(len(tokens) // self.page_size):
+        P, pages, h, at = self.page_size, [], 0, None
+        for i in range(len(tokens) // P):
             h = self._page_hash(h, tokens, i)
-            if h not in self.index:
+            n = self.nodes.get(h)
+            if n is None or n.page < 0 or not n.holds(at, tokens[i * P:(i + 1) * P]):
                 break
-            pages.append(self.index[h])
+            at = n
+            pages.append(n.page)
         self.incref(pages)
-        return pages, len(pages) * self.page_size
+        return pages, len(pages) * P
 
     def insert(self, tokens: list[int], pages: list[int]) -> None:
-        h = 0
-        for i in range(min(len(tokens) // self.page_size, len(pages))):
+        P, h, at = self.page_size, 0, None
+        full = min(len(tokens) // P, len(pages))
+        if any(not 0 <= p < self.num_pages for p in pages[:full]):
+            raise IndexError("page id out of range")
+        for i in range(full):
             h = self._page_hash(h, tokens, i)
-            p = pages[i]
-            if h in self.index or self.cached[p]:
+            n = self.nodes.get(h)
+            if n is None:
+                n = self.nodes[h] = _Node(at, h, list(tokens[i * P:(i + 1) * P]))
+                if at is not None:
+                    at.children += 1
+            elif not n.holds(at, tokens[i * P:(i + 1) * P]):
+                break  # other content with this hash
+            at, p = n, pages[i]
+            if n.page >= 0 or self.node_of[p]:
                 continue
-            self.index[h] = p
-            self.hash_of[p] = h
-            self.cached[p] = True
+            n.page = p
+            self.node_of[p] = n
+        self._trim(at)
 
     def clear_cache(self) -> None:
-        for p in list(self.lru):
-            self.cached[p] = False
-            self.free.append(p)
+        self.free.extend(self.lru)
         self.lru.clear()
-        for p in self.index.values():
-            self.cached[p] = False
-        self.index.clear()
+        self.node_of = [None] * self.num_pages
+        self.nodes.clear()
 
     def stats(self) -> dict:
-        return {"num_pages": self.num_pages, "free": len(self.free), "cached": len(self.index), "evictable": len(self.lru)}
+        return {"num_pages": self.num_pages, "free": len(self.free), "cached": self.num_cached(), "evictable": len(self.lru)}
