@@ -31,6 +31,7 @@ import dataclasses
 import json
 import math
 import os
+import threading
 import time
 import zlib
 from dataclasses import dataclass, field
@@ -193,6 +194,8 @@ class RolloutEngine:
             self.kv = torch.zeros((L, 2, self.num_pages, Hkv, page_size, D), dtype=self.dtype, device=self.device)
         self.preempted: dict[str, _Seq] = {}
         self.bm = make_block_manager(self.num_pages - 1, page_size)
+        # resets of the prefix index so far; a prefill that one overtakes (from another thread) registers nothing
+        self._cache_epoch, self._cache_lock = 0, threading.Lock()
         self.max_pages = math.ceil(max_context / page_size) + 1
         # (the 8-bit decode attention plans for itself)
         self.ws = paged.DecodeWorkspace(max_batch, attn0.nq, max_context + page_size, self.device) if self.is_cuda and self.kv_fp8 is None else None
@@ -546,6 +549,7 @@ class RolloutEngine:
 
     def _prefill(self, groups: list[list[GenRequest]]) -> list[GenResult]:
         t0 = time.perf_counter()
+        epoch = self._cache_epoch
         ids, pos, slots, triples, lasts = [], [], [], [], []
         prefix_slots: list[int] = []  # cached rows that the new ones attend to: the first keys, the new rows' follow
         prefix_triples = []
@@ -618,7 +622,9 @@ class RolloutEngine:
             proto = protos[gi]
             n = len(proto.tokens)
             full = n // self.P
-            self.bm.insert([int(t) for t in proto.tokens], proto.pages)
+            with self._cache_lock:
+                if epoch == self._cache_epoch:
+                    self.bm.insert([int(t) for t in proto.tokens], proto.pages)
             for mi, r in enumerate(members):
                 if mi == 0:
                     s = proto
@@ -741,7 +747,7 @@ class RolloutEngine:
     def release_kv(self) -> None:
         """Give the KV memory back (colocated training phase).  Nothing may be running."""
         assert not self.running, "abort or finish generation before releasing the KV cache"
-        self.bm.clear_cache()
+        self.reset_prefix_cache()
         if self.kv_buf is not None:
             self.kv_buf.pause(backup=False)
 
@@ -1037,5 +1043,8 @@ class RolloutEngine:
             self.reset_prefix_cache()
 
     def reset_prefix_cache(self) -> None:
-        """Weights changed: cached pages no longer match (the reference flushes its radix cache)."""
-        self.bm.clear_cache()
+        """Weights changed: cached pages no longer match (the reference flushes its radix cache).  Nor does a
+        prefill that runs meanwhile register its pages."""
+        with self._cache_lock:
+            self._cache_epoch += 1
+            self.bm.clear_cache()

@@ -70,3 +70,27 @@ def test_calls_of_a_worker_fail_when_a_decode_wait_gave_up(monkeypatch):
             asyncio.run(asyncio.wait_for(worker.generate(inp), 60))
     finally:
         worker.shutdown()
+
+
+# ----------------------------------------------------------------------------- weights that change
+def test_a_prefill_that_a_reset_overtakes_registers_nothing():
+    """The reset comes from another thread while the engine's is inside the forward pass: its rows are of the weights before."""
+    m = _model("cpu")
+    eng = _engine(m, "cpu")
+    p = _prompt(50)
+    assert eng.generate([_greedy("a", p)])[0].cached_tokens == 0
+    layers = eng._layers
+
+    def interrupted(*a, **k):
+        h = layers(*a, **k)
+        eng.reset_prefix_cache()
+        return h
+
+    eng._layers = interrupted
+    eng.generate([_greedy("b", p + _prompt(30, 1), n=1)])
+    eng._layers = layers
+    assert eng.bm.num_cached() == 0 and eng.bm.num_available() == eng.num_pages - 1
+    assert eng.generate([_greedy("c", p)])[0].cached_tokens == 0
+    assert eng.generate([_greedy("d", p)])[0].cached_tokens == 48
+    eng.release_kv()
+    assert eng.generate([_greedy("e", p)])[0].cached_tokens == 0
