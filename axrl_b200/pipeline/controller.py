@@ -212,6 +212,7 @@ class PipelineController:
         if latest_iteration(root) is None:
             return False
         common = load_dist_checkpoint(root, self.train.model, self.train.optim)
+        self.engine.reset_prefix_cache()  # colocated: the engine's weights are the loaded ones
         extra = common.get("extra", {})
         self.global_step = int(extra.get("global_step", common.get("iteration", 0)))
         if self.train_dataset is not None and extra.get("dataset_state"):

@@ -237,6 +237,8 @@ class RolloutEngine:
         from axrl_b200.ops.fp8 import Fp8Weight
 
         self.fp8 = {id(p): Fp8Weight.from_dense(p.detach()) for _, p in self._dense_linear_weights()}
+        if self.kv_fp8 is not None:
+            self.reset_prefix_cache()
 
     def set_fp8_weights(self, weights: dict[str, tuple[torch.Tensor, torch.Tensor]]) -> None:
         """Use externally produced block-fp8 weights (e.g. buffers written by the weight-sync push)."""

@@ -94,3 +94,32 @@ def test_a_prefill_that_a_reset_overtakes_registers_nothing():
     assert eng.generate([_greedy("d", p)])[0].cached_tokens == 48
     eng.release_kv()
     assert eng.generate([_greedy("e", p)])[0].cached_tokens == 0
+
+
+def test_weights_quantised_again_leave_no_cached_prefix():
+    m = _model("cpu")
+    eng = _engine(m, "cpu")
+    p = _prompt(50)
+    eng.generate([_greedy("a", p)])
+    with torch.no_grad():
+        for w in m.parameters():
+            w.mul_(1.01)
+    eng.quantize_weights()
+    assert eng.bm.num_cached() == 0
+
+
+def test_a_loaded_checkpoint_leaves_no_cached_prefix(monkeypatch, tmp_path):
+    """The controller's engine runs on the trainer's weights: what was generated before they are loaded is of other weights."""
+    from types import SimpleNamespace
+
+    from axrl_b200.pipeline.controller import PipelineController
+    from axrl_b200.train import checkpoint
+
+    eng = _engine(_model("cpu"), "cpu")
+    eng.generate([_greedy("a", _prompt(50))])
+    assert eng.bm.num_cached() == 3
+    monkeypatch.setattr(checkpoint, "latest_iteration", lambda root: 7)
+    monkeypatch.setattr(checkpoint, "load_dist_checkpoint", lambda *a: {"iteration": 7})
+    ctl = SimpleNamespace(checkpoint_root=lambda: tmp_path, train=SimpleNamespace(model=eng.model, optim=None), engine=eng, train_dataset=None)
+    assert PipelineController.load_checkpoint_if_existed(ctl)
+    assert ctl.global_step == 7 and eng.bm.num_cached() == 0
