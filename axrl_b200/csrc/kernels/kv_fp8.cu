@@ -66,7 +66,7 @@ struct Cache {
 // each: lane l of 8 holds elements 8l .. 8l + 7 of both halves, so a rotation pair stays in one thread and every access is 16
 // bytes (codes: 8); the next four heads are loaded before the current ones are computed.  16384 tokens of 32 q and 8 kv
 // heads: one warp walking a token with its own angles 100 us, products in registers 113 us (14 warps an SM), this form 79 us,
-// 84 % of the measured copy rate; 2049 tokens of 16 q and 8 kv heads 9.3 us (floor 5.8).
+// 84 % of the measured copy rate; 2049 tokens of 16 q and 8 kv heads 9.4 us (floor 5.8).
 constexpr int AW = 8;  // warps
 
 // Largest magnitude, a NaN if there is one (the sign of the result means nothing).
@@ -948,7 +948,7 @@ __global__ void __launch_bounds__(MW * 32) merge_k(DecParams p) {
 }
 
 // Few short sequences: a CTA per (sequence, kv head), a unit per warp at most, does without the prefix over the lengths and
-// without merge_k.  The block table bounds the lengths.  32 q and 8 kv heads: one sequence of 300 tokens 6.5 against 8.3 us,
+// without merge_k.  The block table bounds the lengths.  32 q and 8 kv heads: one sequence of 300 tokens 6.5 against 8.4 us,
 // 16 of 512 7.2 against 10.1; with more units to a warp the ranges win (one sequence of 2048: 10.0 against 15.3).
 static bool direct_path(int64_t B, int64_t Hkv, int64_t P, int64_t max_pages) { return B * Hkv <= num_sms() && max_pages * P <= DIRECT_TOKENS; }
 
@@ -1015,10 +1015,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> qknorm_rope_cache_fp8(const at::T
   at::Tensor ko, vo;
   if (want_kv) ko = empty_bf16({T, nkv, D}, dev), vo = empty_bf16({T, nkv, D}, dev);
   if (T == 0) return {q, ko, vo};
-  // Warps per token.  Few tokens: eight, for latency (64 tokens of 32 q and 8 kv heads 2.9 us, 5.1 with two).  Many: two, as
-  // many tokens as a CTA then has share its start (16384 tokens 79 us, 85 with four and 107 with eight; 1024 tokens 7.4 us
-  // with eight, 6.8 with four, 11.0 with two), or one where a token has few heads (8 q and 1 kv head, 16384 tokens: 29 us,
-  // 32 with two; 2049 tokens: 8.1 us, 5.3 with two).
+  // Warps per token: the most with which every CTA (eight warps) is resident at once, four on an SM, since the call then takes
+  // as long as one CTA; beyond that two, so that four tokens share a CTA's start, or one where a token has few heads.  32 q and 8 kv
+  // heads, us with 8 / 4 / 2 warps: 64 tokens 3.0 / 3.5 / 5.1, 592 (one wave with eight) 4.5 / 4.4 / 5.3, 593 5.6 / 6.0 / 8.0,
+  // 1184 (one wave with four) 8.1 / 6.4 / 7.0, 1185 8.6 / 7.7 / 10.5, 2368 (one wave with two) 16.2 / 12.5 / 11.8, 9000 57 / 44 / 41.
+  // 8 q and 1 kv head, two warps and one: 2368 tokens 5.3 / 5.6, 4736 9.4 / 8.8, 9000 17.7 / 16.1.
   const int64_t many = (int64_t)num_sms() * 4, groups = (nq + 3) / 4 + (2 * nkv + 3) / 4;
   const int parts = T <= many ? 8 : T <= 2 * many ? 4 : groups < 8 && T > 8 * many ? 1 : 2;
   launch_pdl(append_k, dim3((unsigned)((T + AW / parts - 1) / (AW / parts))), dim3(AW * 32), 0, stream(), (const bf16*)qkv.data_ptr(), (const bf16*)qw.data_ptr(),
